@@ -19,7 +19,9 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from . import oracle, torch_impl
+from . import cache, oracle, torch_impl
+from .cache import CachePlan, KVPages
+from .torch_impl import TokenLogprobs
 
 _BACKEND = os.environ.get("NSA_B200_BACKEND", "auto").lower()
 _native = None
@@ -263,3 +265,71 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor, ignore_
     if _use_native(hidden, "linear_cross_entropy"):
         return native_module().linear_cross_entropy(hidden, weight, labels, ignore_index, chunk)
     return torch_impl.linear_cross_entropy(hidden, weight, labels, ignore_index, chunk)
+
+
+# ------------------------------------------------------------------ generation and scoring
+def cache_pages(pages: int, heads: int, head_dim: int, page_size: int = 64, device=None) -> KVPages:
+    """Empty pages of one layer's 8-bit key / value cache (see :mod:`nsa_optim_b200.ops.cache`)."""
+    return cache.new_pages(pages, heads, head_dim, page_size, device)
+
+
+def _cache_native(t: Tensor) -> bool:
+    """Whether the cache's ops on tensors of whole numbers run as kernels."""
+    return t.is_cuda and _BACKEND != "torch" and native_module() is not None
+
+
+def cache_plan(lengths: Tensor, new: Tensor, table: Tensor, free: Tensor, free_count: Tensor, num_tokens: int,
+               page_size: int) -> CachePlan:
+    """Pages and slots of a step.  Request b holds ``lengths[b]`` tokens and gets ``new[b]`` more (0: it idles), ``num_tokens`` together,
+    packed one request after another (what ``new`` asks for beyond that is left out).  Pages are popped off the stack in the order of the
+    requests and entered into ``table``, in place; entries behind the table's width, or for which the stack has none, count as ``shortfall``,
+    and their tokens have the slot -1: they are neither stored nor seen.  Nothing waits for the device."""
+    if _cache_native(lengths):
+        return native_module().cache_plan(lengths, new, table, free, free_count, num_tokens, page_size)
+    return cache.plan(lengths, new, table, free, free_count, num_tokens, page_size)
+
+
+def cache_release(finished: Tensor, lengths: Tensor, table: Tensor, free: Tensor, free_count: Tensor, page_size: int):
+    """Gives the pages of the requests marked in ``finished`` (B, bool) back to the stack, in place, and clears their rows of ``table``.  Returns
+    (lengths, free_count) after it."""
+    if _cache_native(lengths):
+        return native_module().cache_release(finished, lengths, table, free, free_count, page_size)
+    return cache.release(finished, lengths, table, free, free_count, page_size)
+
+
+def cache_append(pages: KVPages, k: Tensor, v: Tensor, table: Tensor, query_start: Tensor, lengths: Tensor) -> None:
+    """Rounds the keys and values (N, Hkv, D) of a step's packed tokens to 8 bits and stores them, in place, as the last
+    ``query_start[b + 1] - query_start[b]`` of each request's ``lengths[b]`` tokens.  A page's first token sets its scale anew; larger values raise it later,
+    and the page's codes with it.  Tokens without a page are left out."""
+    if _use_native(k, "cache"):
+        return native_module().cache_append(pages, k, v, table, query_start, lengths)
+    return cache.append(pages, k, v, table, query_start, lengths)
+
+
+def cache_values(pages: KVPages, ids: Tensor):
+    """(k, v), each (n, P, Hkv, D) bf16: what whole pages hold, exactly (zeros for an id that is no page; what is behind
+    a page's last token means nothing)."""
+    if _cache_native(ids):
+        return native_module().cache_values(pages, ids)
+    return cache.values(pages, ids)
+
+
+def cache_attention(q: Tensor, pages: KVPages, table: Tensor, query_start: Tensor, lengths: Tensor, window: int = 0,
+                    scale: Optional[float] = None, max_new: int = 1) -> Tensor:
+    """Causal attention of packed queries (N, Hq, D), the last ``query_start[b + 1] - query_start[b]`` of each request's ``lengths[b]`` tokens, over the
+    request's cached keys and values, their own among them (``window`` > 0: the last ``window`` of these alone).  Query heads share KV heads in equal
+    groups.  A query that sees nothing gets zeros.  ``max_new``, the most queries of a request, is a hint for the split of the
+    work: any value gives the same sums up to their order.  Inference only: no gradient is recorded."""
+    if _use_native(q, "cache"):
+        return native_module().cache_attention(q, pages, table, query_start, lengths, window, scale, max_new)
+    return cache.attention(q.detach(), pages, table, query_start, lengths, window, scale)
+
+
+def token_logprobs(logits: Tensor, tokens: Tensor, top_k: int = 0, ignore_index: int = -100) -> TokenLogprobs:
+    """Of logits (..., V): the log probability of each given token (0 where it is ``ignore_index`` or no token), the entropy of each
+    distribution, and the ``top_k`` likeliest tokens with their log probabilities (equal logits: the lower index first), all fp32 and
+    differentiable with respect to the logits.  Tokens whose logit is -inf have probability 0; where no token is left, log
+    probabilities are -inf, the entropy is 0 and no gradient flows."""
+    if logits.is_cuda and _BACKEND != "torch" and logits.dtype in (torch.bfloat16, torch.float32):
+        return native_module().token_logprobs(logits, tokens, top_k, ignore_index)
+    return torch_impl.token_logprobs(logits, tokens, top_k, ignore_index)

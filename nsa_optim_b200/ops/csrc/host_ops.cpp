@@ -39,7 +39,8 @@ using at::Tensor;
   X(nsa_gate_combine_fwd_ex) X(nsa_gate_combine_bwd_ex) X(nsa_pool_fwd) X(nsa_pool_bwd) X(nsa_gdn_prep) X(nsa_gdn_seq_fwd)           \
   X(nsa_gdn_seq_bwd) X(nsa_gdn_post) X(nsa_ssd_states_form) X(nsa_ssd_states) X(nsa_ssd_chunk_state) X(nsa_ssd_state_fwd)         \
   X(nsa_ssd_state_bwd) X(nsa_ssd_chunk_out) X(nsa_ssd_chunk_grad) X(nsa_ssd_grad_slots) X(nsa_ssd_finish) X(nsa_adamw_multi)         \
-  X(nsa_adamw8bit_multi) X(nsa_gates)
+  X(nsa_adamw8bit_multi) X(nsa_gates) X(nsa_cache_plan) X(nsa_cache_release) X(nsa_cache_append) X(nsa_cache_values)                \
+  X(nsa_cache_attention) X(nsa_logprobs_fwd) X(nsa_logprobs_bwd)
 
 struct Lib {
 #define X(f) decltype(&::f) f = nullptr;
@@ -1117,6 +1118,230 @@ OP(adamw8bit) {                                  // items, code books, gradient 
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------- cache
+constexpr auto I64 = at::kLong;
+#define WANT(ok, ...) TORCH_CHECK_VALUE(ok, __VA_ARGS__)
+long long* lp(const Tensor& t) { return static_cast<long long*>(ptr(t)); }
+void want_i32(const Tensor& t, int64_t dims, const char* what, const at::Device& dev) {
+  WANT(t.dim() == dims && t.scalar_type() == I32, what, " has to be an int32 tensor of ", dims, " dimension(s)");
+  WANT(t.device() == dev, what, " is on another device");
+}
+void want_dense(const Tensor& t, const char* what) { WANT(t.is_contiguous(), what, " has to be contiguous: it is changed in place"); }
+void want_page_size(long P) { WANT(P >= 16 && P <= 256 && (P & (P - 1)) == 0, "a page holds a power of two of 16 to 256 tokens, got ", P); }
+int small(int64_t n, const char* what) {
+  WANT(n <= std::numeric_limits<int>::max(), what, " is too large");
+  return static_cast<int>(n);
+}
+
+// The three tensors of a KVPages, as ops/cache.py checks them
+struct Pages {
+  Tensor k, v, scale;
+  int n, H, P, D;
+  static Pages of(Args& a) {
+    Pages p{a.t(), a.t(), a.t(), 0, 0, 0, 0};
+    return p;
+  }
+  void check(const at::Device& dev) {
+    WANT(k.dim() == 6 && v.dim() == 5 && scale.dim() == 3, "expected the three tensors of a KVPages");
+    n = small(k.size(0), "the number of pages");
+    H = small(k.size(1), "the number of heads");
+    P = small(2 * k.size(2), "a page");
+    D = small(64 * k.size(3), "head_dim");
+    want_page_size(P);
+    WANT(k.size(4) == 2 && k.size(5) == 64 && v.sizes() == at::IntArrayRef({n, H, P / 16, D, 16}) && scale.sizes() == at::IntArrayRef({n, H, 2}),
+         "the shapes of a KVPages do not belong together");
+    WANT(k.scalar_type() == at::kByte && v.scalar_type() == at::kByte && scale.scalar_type() == F32, "a KVPages is uint8, uint8 and float32");
+    WANT(k.is_contiguous() && v.is_contiguous() && scale.is_contiguous(), "the tensors of a KVPages have to be contiguous");
+    WANT(k.device() == dev && v.device() == dev && scale.device() == dev, "the pages are on another device");
+    WANT(aligned(k) && aligned(v) && reinterpret_cast<uintptr_t>(scale.data_ptr()) % 8 == 0, "the tensors of a KVPages have to be 16-byte aligned");
+  }
+};
+
+// Tables and lengths of a step's requests
+struct Step {
+  Tensor table, start, lengths;
+  static Step of(Args& a) { return Step{a.t(), a.t(), a.t()}; }
+  void check(const at::Device& dev) {
+    want_i32(table, 2, "table", dev);
+    want_i32(start, 1, "query_start", dev);
+    want_i32(lengths, 1, "lengths", dev);
+    WANT(B() > 0 && table.size(0) == B() && start.size(0) == B() + 1, "table, query_start and lengths have to be of the same requests");
+    table = table.contiguous();
+    start = start.contiguous();
+    lengths = lengths.contiguous();
+  }
+  int B() const { return dim(lengths.size(0)); }
+  int W() const { return dim(table.size(1)); }
+};
+
+// (N, H, D) whose heads and columns are dense and whose tokens' rows are 16-byte aligned, of any pitch
+Tensor packed_rows(const Tensor& t) {
+  const bool ok = t.stride(2) == 1 && t.stride(1) == t.size(2) && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) * t.size(2) && aligned(t);
+  return ok ? t : at::empty(t.sizes(), t.options()).copy_(t);
+}
+
+OP(cache_plan) {                                 // lengths, new, table, free, free_count, tokens, page size -> the fields of a CachePlan
+  return entry(py, np, [](Args& a) {
+    const Tensor &lengths = a.t(), &add = a.t(), &table = a.t(), &pages = a.t(), &count = a.t();
+    const long N = a.count(), P = a.count();
+    return [=]() -> List {
+      const auto dev = lengths.device();
+      want_i32(lengths, 1, "lengths", dev);
+      want_i32(add, 1, "new", dev);
+      want_i32(table, 2, "table", dev);
+      want_i32(pages, 1, "free", dev);
+      want_i32(count, 1, "free_count", dev);
+      want_page_size(P);
+      const int64_t B = table.size(0), W = table.size(1);
+      WANT(B > 0 && W > 0 && lengths.size(0) == B && add.size(0) == B, "lengths, new and table have to be of the same requests");
+      WANT(count.size(0) == 1 && N >= 0, "free_count has one element, num_tokens is not negative");
+      want_dense(table, "table");
+      const Tensor l = lengths.contiguous(), n = add.contiguous(), f = pages.contiguous();
+      const Tensor start = alloc({B + 1}, I32, dev), total = alloc({B}, I32, dev), slots = alloc({N}, I64, dev), at = alloc({N}, I64, dev);
+      const Tensor left = alloc({1}, I32, dev), lack = alloc({1}, I32, dev);
+      launch(lib.nsa_cache_plan, ip(l), ip(n), ip(table), ip(f), ip(count), small(f.numel(), "the stack"), ip(start), ip(total), lp(slots), lp(at),
+             ip(left), ip(lack), small(B, "the number of requests"), small(W, "table"), small(N, "num_tokens"), dim(P));
+      return {start, total, slots, at, left, lack};
+    };
+  });
+}
+
+OP(cache_release) {                              // finished, lengths, table, free, free_count, page size -> lengths, free_count
+  return entry(py, np, [](Args& a) {
+    const Tensor &done = a.t(), &lengths = a.t(), &table = a.t(), &pages = a.t(), &count = a.t();
+    const long P = a.count();
+    return [=]() -> List {
+      const auto dev = lengths.device();
+      want_i32(lengths, 1, "lengths", dev);
+      want_i32(table, 2, "table", dev);
+      want_i32(pages, 1, "free", dev);
+      want_i32(count, 1, "free_count", dev);
+      want_page_size(P);
+      const int64_t B = table.size(0), W = table.size(1);
+      WANT(done.scalar_type() == at::kBool && done.dim() == 1 && done.size(0) == B && done.device() == dev && lengths.size(0) == B &&
+               count.size(0) == 1 && B > 0 && W > 0,
+           "finished is a truth value for each request, free_count has one element");
+      want_dense(table, "table");
+      want_dense(pages, "free");
+      const Tensor d = done.contiguous(), l = lengths.contiguous(), total = alloc({B}, I32, dev), left = alloc({1}, I32, dev);
+      launch(lib.nsa_cache_release, static_cast<const void*>(ptr(d)), ip(l), ip(table), ip(pages), ip(count), small(pages.numel(), "the stack"),
+             ip(total), ip(left), small(B, "the number of requests"), small(W, "table"), dim(P));
+      return {total, left};
+    };
+  });
+}
+
+OP(cache_append) {                               // k, v, pages, step -> nothing
+  return entry(py, np, [](Args& a) {
+    const Tensor &k_ = a.t(), &v_ = a.t();
+    Pages p = Pages::of(a);
+    Step s = Step::of(a);
+    return [=]() mutable -> List {
+      const auto dev = k_.device();
+      p.check(dev);
+      s.check(dev);
+      WANT(k_.dim() == 3 && k_.sizes() == v_.sizes() && k_.size(1) == p.H && k_.size(2) == p.D && k_.scalar_type() == BF &&
+               v_.scalar_type() == BF && v_.device() == dev,
+           "keys and values have to be (tokens, ", p.H, ", ", p.D, ") and of one type, got ", k_.sizes(), " and ", v_.sizes());
+      const Tensor k = packed_rows(k_), v = packed_rows(v_);
+      launch(lib.nsa_cache_append, static_cast<const void*>(ptr(k)), static_cast<const void*>(ptr(v)), k.stride(0), v.stride(0), ptr(p.k), ptr(p.v),
+             fp(p.scale), ip(s.table), ip(s.start), ip(s.lengths), s.B(), s.W(), small(k.size(0), "the number of tokens"), p.n, p.H, p.D, p.P);
+      return {};
+    };
+  });
+}
+
+OP(cache_values) {                               // pages, ids -> k, v
+  return entry(py, np, [](Args& a) {
+    Pages p = Pages::of(a);
+    const Tensor& ids = a.t();
+    return [=]() mutable -> List {
+      const auto dev = ids.device();
+      p.check(dev);
+      want_i32(ids, 1, "ids", dev);
+      const int64_t n = ids.size(0);
+      const Tensor i = ids.contiguous(), k = alloc({n, p.P, p.H, p.D}, BF, dev), v = alloc({n, p.P, p.H, p.D}, BF, dev);
+      launch(lib.nsa_cache_values, static_cast<const void*>(ptr(p.k)), static_cast<const void*>(ptr(p.v)), fp(p.scale), ip(i), ptr(k), ptr(v),
+             small(n, "the number of pages"), p.n, p.H, p.D, p.P);
+      return {k, v};
+    };
+  });
+}
+
+OP(cache_attention) {                            // q, pages, step, window, scale, max_new -> o
+  return entry(py, np, [](Args& a) {
+    const Tensor& q_ = a.t();
+    Pages p = Pages::of(a);
+    Step s = Step::of(a);
+    const long window = a.count();
+    const float scale = a.f();
+    const long most = a.count();
+    return [=]() mutable -> Tensor {
+      const auto dev = q_.device();
+      p.check(dev);
+      s.check(dev);
+      WANT(q_.dim() == 3 && q_.size(2) == p.D && q_.size(1) > 0 && q_.size(1) % p.H == 0, "queries have to be (tokens, a multiple of ", p.H,
+           " heads, ", p.D, "), got ", q_.sizes());
+      WANT(window >= 0, "window has to be 0 (none) or more");
+      const Tensor q = packed_rows(q_), o = alloc(q.sizes(), BF, dev);
+      const long far = std::numeric_limits<int>::max();
+      launch(lib.nsa_cache_attention, static_cast<const void*>(ptr(q)), q.stride(0), static_cast<const void*>(ptr(p.k)),
+             static_cast<const void*>(ptr(p.v)), fp(p.scale), ip(s.table), ip(s.start), ip(s.lengths), ptr(o), s.B(), s.W(),
+             small(q.size(0), "the number of tokens"), p.n, small(q.size(1), "the number of heads"), p.H, p.D, p.P,
+             window < far ? dim(window) : 0, scale, dim(most < 1 ? 1 : most < far ? most : far));
+      return o;
+    };
+  });
+}
+
+// ------------------------------------------------------------------------------------- log probabilities
+// (rows, V) of uniform pitch without a copy where it can be
+Tensor logit_rows(const Tensor& t) {
+  const int64_t V = t.size(-1);
+  if (t.is_contiguous()) return t.view({-1, V});
+  if (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= V) return t;
+  return t.contiguous().view({-1, V});
+}
+
+OP(logprobs_fwd) {                               // logits, tokens, k, ignored token -> logprob, entropy, top, index, stats, logits' rows, tokens
+  return entry(py, np, [](Args& a) {
+    const Tensor &x_ = a.t(), &tok = a.t();
+    const long k = a.count(), ignore = a.count();
+    return [=]() -> List {
+      WANT(x_.dim() >= 1 && x_.size(-1) >= 1, "logits have to be (..., V) floating-point numbers, V at least 1");
+      const auto dev = x_.device();
+      const auto shape = x_.sizes().slice(0, x_.dim() - 1);
+      WANT(tok.scalar_type() == I64 && tok.sizes() == shape && tok.device() == dev, "tokens have to be int64 of the shape ", shape,
+           " and on the device of the logits");
+      const int64_t V = x_.size(-1), n = tok.numel();
+      WANT(k >= 0 && k <= V, "top_k has to be 0 to ", V, ", got ", k);
+      std::vector<int64_t> wide(shape.begin(), shape.end());
+      wide.push_back(k);
+      const Tensor x = n ? logit_rows(x_) : x_.reshape({0, V}), t = tok.contiguous();
+      const Tensor lp_ = alloc(shape, F32, dev), H = alloc(shape, F32, dev), stats = alloc({n, 2}, F32, dev), top = alloc(wide, F32, dev), at = alloc(wide, I64, dev);
+      launch(lib.nsa_logprobs_fwd, static_cast<const void*>(ptr(x)), x.stride(0), static_cast<int>(x.scalar_type() == F32), lp(t), fp(lp_), fp(H),
+             fp(stats), fp(top), lp(at), static_cast<long>(n), small(V, "the vocabulary"), dim(k), static_cast<long long>(ignore));
+      return {lp_, H, top, at, stats, x, t};
+    };
+  });
+}
+
+OP(logprobs_bwd) {                               // logits' rows, tokens, stats, entropy, index, d logprob, d entropy, d top (each or None), ignored, shape -> dx
+  return entry(py, np, [](Args& a) {
+    const Tensor &x = a.t(), &tok = a.t(), &stats = a.t(), &H = a.t(), &at = a.t();
+    const Tensor g_ = a.opt(), gH_ = a.opt(), gt_ = a.opt();
+    const long ignore = a.count();
+    return [=]() -> Tensor {
+      auto f32 = [](const Tensor& t) { return t.defined() ? to(t, F32).contiguous() : t; };
+      const Tensor g = f32(g_), gH = f32(gH_), gt = f32(gt_), dx = alloc(x.sizes(), x.scalar_type(), x.device());
+      const int k = dim(at.size(-1));
+      launch(lib.nsa_logprobs_bwd, static_cast<const void*>(ptr(x)), row_pitch(x), static_cast<int>(x.scalar_type() == F32), lp(tok), fp(stats), fp(H), lp(at),
+             fp(g), fp(gH), fp(gt), ptr(dx), static_cast<long>(x.size(0)), dim(x.size(1)), k, static_cast<long long>(ignore));
+      return dx;
+    };
+  });
+}
+
 // ------------------------------------------------------------------------------------- the module
 OP(bind) {                                       // path of the library, the dictionary of ops/native.py, most parts of a split reduction
   HANDLE_TH_ERRORS
@@ -1161,6 +1386,7 @@ PyMethodDef methods[] = {
     M(swiglu_fwd), M(swiglu_bwd), M(rope), M(conv_fwd), M(conv_bwd), M(embedding_fwd), M(matmul), M(linear_fwd), M(multi_linear_fwd),
     M(multi_linear_bwd), M(cross_entropy_fwd), M(scale), M(attn_fwd), M(attn_bwd), M(union_blocks), M(inverse_blocks), M(importance), M(select),
     M(gates_fwd), M(gates_bwd), M(pool_fwd), M(pool_bwd), M(nsa_bwd), M(gdn_fwd), M(gdn_bwd), M(ssd_fwd), M(ssd_bwd), M(gates), M(adamw), M(adamw8bit),
+    M(cache_plan), M(cache_release), M(cache_append), M(cache_values), M(cache_attention), M(logprobs_fwd), M(logprobs_bwd),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_nsa_host", "Host side of the native ops.", -1, methods};
 }  // namespace

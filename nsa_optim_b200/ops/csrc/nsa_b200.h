@@ -211,6 +211,30 @@ int nsa_affine_dequant(const uint8_t* q, const float* scale, const float* zero, 
 int nsa_copy2d(void* dst, long dst_pitch_bytes, const void* src, long src_pitch_bytes, long width_bytes, long rows,
     cudaStream_t st);
 
+/* ---- cache.cu, cache_attention.cu: a paged key / value cache in 8 bits (layout: ops/cache.py) ---- */
+/* Pages and slots of a step of N tokens; table is changed in place.  At most nsa_cache_plan_limit() requests. */
+int nsa_cache_plan(const int* lengths, const int* add, int* table, const int* free_pages, const int* free_count, int F, int* query_start,
+    int* total, long long* slots, long long* positions, int* free_left, int* shortfall, int B, int W, int N, int page_size, cudaStream_t st);
+int nsa_cache_plan_limit(void);
+int nsa_cache_release(const void* finished, const int* lengths, int* table, int* free_pages, const int* free_count, int F, int* total,
+    int* free_left, int B, int W, int page_size, cudaStream_t st);
+/* bf16 (N, H, D) rows of pitch ldk, ldv into the pages of their requests */
+int nsa_cache_append(const void* k, const void* v, long ldk, long ldv, void* kc, void* vc, float* scale, const int* table, const int*
+    query_start, const int* lengths, int B, int W, int N, int pages, int H, int D, int page_size, cudaStream_t st);
+int nsa_cache_values(const void* kc, const void* vc, const float* scale, const int* ids, void* k, void* v, int n, int pages, int H, int D,
+    int page_size, cudaStream_t st);
+int nsa_cache_attention(const void* q, long ldq, const void* kc, const void* vc, const float* scale, const int* table, const int*
+    query_start, const int* lengths, void* o, int B, int W, int N, int pages, int Hq, int H, int D, int page_size, int window, float
+    softmax_scale, int max_new, cudaStream_t st);
+
+/* ---- logprobs.cu: rows of bf16 or fp32 logits of pitch ld; entropies; stats: maximum and log of the
+ * sum above it, 8-byte aligned; the k likeliest tokens ---- */
+int nsa_logprobs_fwd(const void* logits, long ld, int fp32, const long long* tokens, float* logprob, float* entropy, float* stats, float*
+    top, long long* index, long rows, int V, int k, long long ignore, cudaStream_t st);
+int nsa_logprobs_bwd(const void* logits, long ld, int fp32, const long long* tokens, const float* stats, const float* entropy, const long
+    long* index, const float* dlogprob, const float* dentropy, const float* dtop, void* dx, long rows, int V, int k, long long ignore,
+    cudaStream_t st);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,7 +20,7 @@ import torch
 from torch import Tensor
 from torch.autograd import forward_ad
 
-from . import quant, torch_impl
+from . import cache, quant, torch_impl
 from .signatures import declare
 
 _LIB_PATH = os.environ.get("NSA_B200_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libnsa_b200.so")
@@ -31,7 +31,7 @@ _SPLITK_MAX = int(os.environ.get("NSA_B200_SPLITK_MAX", "2"))
 SUPPORTED = {
     "linear", "rms_norm", "gated_rms_norm", "swiglu", "l2_norm", "rope", "embedding",
     "causal_conv1d", "linear_cross_entropy", "adamw", "adamw_lowbit", "gated_delta_rule",
-    "attention", "nsa_attention", "ssd_scan",
+    "attention", "nsa_attention", "ssd_scan", "cache", "token_logprobs",
 }
 
 STATUS_NAMES = {
@@ -117,7 +117,7 @@ class _NoRecord:
     def save_for_backward(self, *tensors):
         pass
 
-    mark_non_differentiable = save_for_backward
+    mark_non_differentiable = set_materialize_grads = save_for_backward
 
 
 def _recorded(args) -> bool:
@@ -1212,3 +1212,52 @@ def _ssd_scan_batched(x, dt, A, Bm, Cm, D=None, chunk=256):
     if D is not None:
         y = y + (x[:, :T].float() * D.float()[None, None, :, None]).to(cdt)
     return y.to(cdt)
+
+
+# --------------------------------------------------------------------------------------
+# generation and scoring (csrc/cache.cu, csrc/cache_attention.cu, csrc/logprobs.cu)
+# --------------------------------------------------------------------------------------
+def cache_plan(lengths, new, table, free, free_count, num_tokens, page_size):
+    if lengths.shape[:1].numel() > 16384:                      # one CTA holds a number for each request
+        _fallback("cache_plan")
+        return cache.plan(lengths, new, table, free, free_count, num_tokens, page_size)
+    return cache.CachePlan(*_h().cache_plan(lengths, new, table, free, free_count, num_tokens, page_size))
+
+
+def cache_release(finished, lengths, table, free, free_count, page_size):
+    return _h().cache_release(finished, lengths, table, free, free_count, page_size)
+
+
+def cache_append(pages, k, v, table, query_start, lengths):
+    _h().cache_append(k, v, *pages, table, query_start, lengths)
+
+
+def cache_values(pages, ids):
+    return _h().cache_values(*pages, ids)
+
+
+def cache_attention(q, pages, table, query_start, lengths, window=0, scale=None, max_new=1):
+    D = q.shape[-1]
+    if D not in (64, 128):
+        _fallback("cache_attention")
+        return cache.attention(q.detach(), pages, table, query_start, lengths, window, scale)
+    return _h().cache_attention(q, *pages, table, query_start, lengths, window, D ** -0.5 if scale is None else scale, max_new)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top_k, ignore_index):
+        logprob, entropy, top, index, stats, x, tok = _h().logprobs_fwd(logits, tokens, top_k, ignore_index)
+        ctx.save_for_backward(x, tok, stats, entropy, index)
+        ctx.shape, ctx.ignore = logits.shape, ignore_index
+        ctx.mark_non_differentiable(index)
+        ctx.set_materialize_grads(False)
+        return logprob, entropy, top, index
+
+    @staticmethod
+    def backward(ctx, dlogprob, dentropy, dtop, _dindex):
+        return _host.logprobs_bwd(*ctx.saved_tensors, dlogprob, dentropy, dtop, ctx.ignore).view(ctx.shape), None, None, None
+
+
+def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
+    return torch_impl.TokenLogprobs(*_run(_TokenLogprobs, logits, tokens, top_k, ignore_index))

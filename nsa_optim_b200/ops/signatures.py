@@ -24,6 +24,12 @@ SIGNATURES = {
     "nsa_attn_bwd_walks_d64": "iiiiiiiii",
     "nsa_attn_fwd": "ipppppiiiiiifiiiipppip",
     "nsa_attn_importance": "ippppiiiiiifiiip",
+    "nsa_cache_append": "ippllppppppiiiiiiip",
+    "nsa_cache_attention": "iplpppppppiiiiiiiiifip",
+    "nsa_cache_plan": "ipppppippppppiiiip",
+    "nsa_cache_plan_limit": "i",
+    "nsa_cache_release": "ipppppippiiip",
+    "nsa_cache_values": "ippppppiiiiip",
     "nsa_comm_allgather": "ippliipuqip",
     "nsa_comm_reduce_scatter": "ippliifippuqp",
     "nsa_comm_reduce_scatter_parts": "i",
@@ -63,6 +69,8 @@ SIGNATURES = {
     "nsa_last_error": "s",
     "nsa_launch_count": "q",
     "nsa_launch_count_reset": "v",
+    "nsa_logprobs_bwd": "iplippppppppliiqp",
+    "nsa_logprobs_fwd": "iplippppppliiqp",
     "nsa_mamba3_scan": "ipppppppiiiip",
     "nsa_pool_bwd": "ippiiiiip",
     "nsa_pool_fwd": "ippiiiliip",

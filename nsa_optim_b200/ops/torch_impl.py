@@ -18,7 +18,7 @@ Chunked algorithms implemented here:
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -405,3 +405,41 @@ class _LinearCrossEntropy(torch.autograd.Function):
 def linear_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor, ignore_index: int = -100,
                          chunk: int = 4096) -> Tensor:
     return _LinearCrossEntropy.apply(hidden, weight, labels, ignore_index, chunk)
+
+
+# ------------------------------------------------------------------ log probabilities
+class TokenLogprobs(NamedTuple):
+    """Results of ``ops.token_logprobs``, fp32 but for the int64 ``top_index``."""
+    logprob: Tensor
+    entropy: Tensor
+    top_logprob: Tensor
+    top_index: Tensor
+
+
+def check_token_logprobs(logits: Tensor, tokens: Tensor, top_k: int) -> None:
+    if logits.dim() < 1 or logits.shape[-1] < 1 or not logits.is_floating_point():
+        raise ValueError("logits have to be (..., V) floating-point numbers, V at least 1")
+    if tokens.dtype != torch.long or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"tokens have to be int64 of the shape {tuple(logits.shape[:-1])}, got {tokens.dtype} {tuple(tokens.shape)}")
+    if not 0 <= top_k <= logits.shape[-1]:
+        raise ValueError(f"top_k has to be 0 to {logits.shape[-1]}, got {top_k}")
+
+
+def token_logprobs(logits: Tensor, tokens: Tensor, top_k: int = 0, ignore_index: int = -100) -> TokenLogprobs:
+    check_token_logprobs(logits, tokens, top_k)
+    x = logits.float()
+    m = x.detach().amax(-1, keepdim=True)
+    empty = torch.isneginf(m)                                  # nothing may follow: log probabilities of -inf, no entropy, no gradient
+    below = torch.where(empty, x.detach(), x - torch.where(empty, 0.0, m))
+    e = below.exp()
+    S = torch.where(empty, 1.0, e.sum(-1, keepdim=True))
+    logp = below - S.log()
+    p = e / S
+    gone = torch.isneginf(x)
+    entropy = -(p * torch.where(gone, 0.0, logp)).masked_fill(gone, 0.0).sum(-1)
+    counts = (tokens != ignore_index) & (tokens >= 0) & (tokens < x.shape[-1])
+    chosen = logp.gather(-1, torch.where(counts, tokens, 0).unsqueeze(-1)).squeeze(-1)
+    chosen = torch.where(counts, chosen, 0.0)
+    # a stable sort: equal logits in the order of their indices, NaN first
+    top = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
+    return TokenLogprobs(chosen, entropy, logp.gather(-1, top), top)
