@@ -40,7 +40,7 @@ using at::Tensor;
   X(nsa_gdn_seq_bwd) X(nsa_gdn_post) X(nsa_ssd_states_form) X(nsa_ssd_states) X(nsa_ssd_chunk_state) X(nsa_ssd_state_fwd)         \
   X(nsa_ssd_state_bwd) X(nsa_ssd_chunk_out) X(nsa_ssd_chunk_grad) X(nsa_ssd_grad_slots) X(nsa_ssd_finish) X(nsa_adamw_multi)         \
   X(nsa_adamw8bit_multi) X(nsa_gates) X(nsa_cache_plan) X(nsa_cache_release) X(nsa_cache_append) X(nsa_cache_values)                \
-  X(nsa_cache_attention) X(nsa_logprobs_fwd) X(nsa_logprobs_bwd)
+  X(nsa_cache_attention) X(nsa_cache_attention_scratch) X(nsa_logprobs_fwd) X(nsa_logprobs_bwd)
 
 struct Lib {
 #define X(f) decltype(&::f) f = nullptr;
@@ -1285,10 +1285,11 @@ OP(cache_attention) {                            // q, pages, step, window, scal
       WANT(window >= 0, "window has to be 0 (none) or more");
       const Tensor q = packed_rows(q_), o = alloc(q.sizes(), BF, dev);
       const long far = std::numeric_limits<int>::max();
+      const int new_ = dim(most < 1 ? 1 : most < far ? most : far), Hq = small(q.size(1), "the number of heads");
+      const Tensor scratch = alloc({have(lib.nsa_cache_attention_scratch)(Hq, p.H, p.D, new_)}, F32, dev);
       launch(lib.nsa_cache_attention, static_cast<const void*>(ptr(q)), q.stride(0), static_cast<const void*>(ptr(p.k)),
-             static_cast<const void*>(ptr(p.v)), fp(p.scale), ip(s.table), ip(s.start), ip(s.lengths), ptr(o), s.B(), s.W(),
-             small(q.size(0), "the number of tokens"), p.n, small(q.size(1), "the number of heads"), p.H, p.D, p.P,
-             window < far ? dim(window) : 0, scale, dim(most < 1 ? 1 : most < far ? most : far));
+             static_cast<const void*>(ptr(p.v)), fp(p.scale), ip(s.table), ip(s.start), ip(s.lengths), ptr(o), fp(scratch), s.B(),
+             s.W(), small(q.size(0), "the number of tokens"), p.n, Hq, p.H, p.D, p.P, window < far ? dim(window) : 0, scale, new_);
       return o;
     };
   });

@@ -223,8 +223,10 @@ int nsa_cache_append(const void* k, const void* v, long ldk, long ldv, void* kc,
     query_start, const int* lengths, int B, int W, int N, int pages, int H, int D, int page_size, cudaStream_t st);
 int nsa_cache_values(const void* kc, const void* vc, const float* scale, const int* ids, void* k, void* v, int n, int pages, int H, int D,
     int page_size, cudaStream_t st);
+/* scratch: nsa_cache_attention_scratch(...) floats, 16-byte aligned */
+long nsa_cache_attention_scratch(int Hq, int H, int D, int max_new);
 int nsa_cache_attention(const void* q, long ldq, const void* kc, const void* vc, const float* scale, const int* table, const int*
-    query_start, const int* lengths, void* o, int B, int W, int N, int pages, int Hq, int H, int D, int page_size, int window, float
+    query_start, const int* lengths, void* o, float* scratch, int B, int W, int N, int pages, int Hq, int H, int D, int page_size, int window, float
     softmax_scale, int max_new, cudaStream_t st);
 
 /* ---- logprobs.cu: rows of bf16 or fp32 logits of pitch ld; entropies; stats: maximum and log of the
