@@ -9,22 +9,29 @@
 //  * Each worker has its own ring of key and value tiles that bulk copies fill two tiles ahead: 130 KB in flight per SM, no registers, and no
 //    synchronisation between workers.
 //  * The cache's orders are those of the product's operands.  Of a unit, lane 4c+r of a warp scores token 2j + c%2 of sub-block c/2 in tile j and holds
-//    the probabilities of sub-block r's tokens 2j, 2j+1, so its value operand is 16 neighbouring bytes; a code becomes f16 by a byte permutation and one subtraction.
-//  * f16 holds a code exactly, and a query row scaled by a power of two to 2^13 .. 2^14 (bf16's 8 bits; what is 2^-28 of the row's largest
-//    value rounds).  Probabilities are rounded to 11 bits, relative to the row's largest product of probability and value scale: the value scale's
-//    exponent is added to x, and taken out again of the sum.  Sums are fp32.
+//    the probabilities of sub-block r's tokens 2j, 2j+1, so its value operand is 16 neighbouring bytes.
+//  * A code u becomes an f16 operand by a byte permutation alone: the bits 0x00uu are the (subnormal) number 2^-24 u.  The offset of 128 comes out
+//    of sums: 128 sum(q) of a row's scores, and 128 sum(p) of its outputs, which one more product per step leaves in the accumulators' format and
+//    which is taken off every fourth unit, before it outgrows them.  (With a subtraction per pair of codes, 256 of 1170 instructions a unit, 64
+//    contexts of up to 8192 tokens took XX us.)
+//  * Codes and their products are exact, and so is a query row scaled by a power of two to 2^13 .. 2^14 (bf16's 8 bits; what is 2^-28 of the row's
+//    largest value rounds).  Probabilities are rounded to 11 bits, relative to the row's largest product of probability and value scale: the value
+//    scale's exponent is added to x, and taken out again of the sum.  Sums are fp32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
 
+#include <atomic>
+
 #include "cache.cuh"
+#include "f32x2.cuh"
 #include "host.cuh"
 #include "tc5.cuh"
 
 namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kMaxRequests = 1024;                       // of one launch: their prefix sums are in shared memory
+constexpr int kMaxRequests = 768;                        // of one launch: their prefix sums are in shared memory
 
 struct AttnParams {
   const bf16* q;
@@ -35,10 +42,17 @@ struct AttnParams {
   float* head;          // (CTA, worker, rows, D): parts of requests that end inside a worker's range and began before it
   float* part;          // (CTA, 2, rows, D): parts of requests that go beyond a CTA: one that began before it, one that goes on behind it
   float2* part_ml;      // (CTA, 2, rows)
-  int4* join;           // (CTA): request, KV head and first row that begin in the CTA and end in CTA .w; .w = 0: none
+  struct Join* join;    // (CTA)
   int Hq, G, window;
+  unsigned long long per_g;   // ceil(2^32 / G): row / G of rows below 2^32 / G is a multiplication
   float scale;          // times log2(e)
   KernelStatus* status;
+};
+
+// The item that begins in a CTA and ends in another, if there is one
+struct Join {
+  int any, b, h, row0;
+  long long end, each;  // the unit at which it ends, units of a worker
 };
 
 template <int D, int MT>
@@ -51,13 +65,23 @@ struct Shape {
   static_assert(kRing >= kRows * D * 4, "a worker's sums go where its ring was");
 };
 
+__device__ __forceinline__ int token_of(const AttnParams& p, int row) { return static_cast<int>(static_cast<unsigned>(row) * p.per_g >> 32); }
+
 // What a worker has left in memory at the end
 struct Left {
   int head, tail;       // whether there is a part that began before the range and ended in it; whether the last part is open at either end
   int began, open;      // of the last part: began before the range; goes on behind it
   int head_item[3], tail_item[3];                                      // request, KV head, first row
-  int tail_last;        // the CTA in which the last part's item ends
+  long long tail_end;   // the unit at which the last part's item ends
   int some;             // the range is not empty
+};
+
+struct Request {
+  int n, q0;            // queries, the first one's row in q
+  int past, cap;        // tokens before them, keys that the table can hold
+  // 64-key units that any of them sees
+  __device__ __forceinline__ int unit0(int window) const { return window > 0 ? max(past - window + 1, 0) >> 6 : 0; }
+  __device__ __forceinline__ int units(int window) const { return n > 0 ? max(((cap + 63) >> 6) - unit0(window), 1) : 0; }
 };
 
 template <int D, int MT>
@@ -69,16 +93,12 @@ struct Smem {
   float2 ml[S::kGroups][2][S::kRows];
   Left left[S::kGroups];
   long long before[kMaxRequests + 1];                                  // units of the requests before b
+  Request request[kMaxRequests];
   long long warps[kWarps];
   int abort_flag;
 };
 
 // ------------------------------------------------------------------------------------- work
-struct Request {
-  int n, q0;            // queries, the first one's row in q
-  int past, cap;        // tokens before them, keys that the table can hold
-  int unit0, units;     // 64-key units that any of them sees
-};
 __device__ __forceinline__ Request request_of(const AttnParams& p, int b) {
   Request r;
   const int lo = p.s.query_start[b], hi = p.s.query_start[b + 1], len = p.s.lengths[b];
@@ -86,8 +106,6 @@ __device__ __forceinline__ Request request_of(const AttnParams& p, int b) {
   r.n = max(min(hi, p.s.N) - r.q0, 0);
   r.past = len - (hi - lo);
   r.cap = static_cast<int>(min(static_cast<long long>(max(len, 0)), static_cast<long long>(p.s.W) << p.c.shift));
-  r.unit0 = p.window > 0 ? max(r.past - p.window + 1, 0) >> 6 : 0;
-  r.units = r.n > 0 ? max(((r.cap + 63) >> 6) - r.unit0, 1) : 0;
   return r;
 }
 
@@ -101,20 +119,41 @@ struct Piece {
 
 template <int ROWS>
 struct Cursor {
-  long long at, end;
-  int b;
+  long long at, end;    // the range that is left
+  int b, h, tile, first;                                               // the item in which it begins, and its unit
   Piece p;
 
+  __device__ __forceinline__ void init(const AttnParams& a, const long long* before, const Request* request, long long from, long long to) {
+    at = from;
+    end = to;
+    int lo = 0, hi = a.s.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] <= at) lo = mid; else hi = mid;
+    }
+    b = lo;
+    h = tile = first = 0;
+    if (at < end) {
+      const int units = request[b].units(a.window), tiles = (request[b].n * a.G + ROWS - 1) / ROWS;
+      unsigned long long rel = at - before[b], item;
+      if (rel >> 32) {
+        item = rel / units;
+        h = static_cast<int>(item / tiles);
+      } else {
+        item = static_cast<unsigned>(rel) / static_cast<unsigned>(units);
+        h = static_cast<int>(static_cast<unsigned>(item) / static_cast<unsigned>(tiles));
+      }
+      tile = static_cast<int>(item - static_cast<unsigned long long>(h) * tiles);
+      first = static_cast<int>(rel - item * units);
+    }
+  }
+
   // The next piece of the range; false at its end
-  __device__ __forceinline__ bool next_piece(const AttnParams& a, const long long* before) {
+  __device__ __forceinline__ bool next_piece(const AttnParams& a, const long long* before, const Request* request) {
     if (at >= end) return false;
-    while (before[b + 1] <= at) ++b;
-    const Request r = request_of(a, b);
-    const int tiles = (r.n * a.G + ROWS - 1) / ROWS;
-    const long long rel = at - before[b], item = rel / r.units;
-    const int h = static_cast<int>(item / tiles), tile = static_cast<int>(item - static_cast<long long>(h) * tiles);
-    const int first = static_cast<int>(rel - item * r.units);
-    const long long item_at = before[b] + item * r.units, stop = min(item_at + r.units, end);
+    const Request r = request[b];
+    const int units = r.units(a.window), tiles = (r.n * a.G + ROWS - 1) / ROWS, rest = units - first;
+    const int count = static_cast<int>(min(static_cast<long long>(rest), end - at));
     p.b = b;
     p.h = h;
     p.row0 = tile * ROWS;
@@ -123,15 +162,27 @@ struct Cursor {
     p.past = r.past;
     p.cap = r.cap;
     p.began = first > 0;
-    p.open = stop < item_at + r.units;
-    p.item_end = item_at + r.units;
+    p.open = count < rest;
+    p.item_end = at + rest;
     // units that some row of the tile sees
-    const int t0 = p.row0 / a.G, t1 = min((p.row0 + ROWS - 1) / a.G, r.n - 1);
+    const int t0 = token_of(a, p.row0), t1 = min(token_of(a, p.row0 + ROWS - 1), r.n - 1), unit0 = r.unit0(a.window);
     const int from = a.window > 0 ? max(r.past + t0 - a.window + 1, 0) >> 6 : 0;
     const int to = min(r.past + t1 >= 0 ? ((r.past + t1) >> 6) + 1 : 0, (r.cap + 63) >> 6);
-    p.lo = max(r.unit0 + first, from);
-    p.hi = min(r.unit0 + static_cast<int>(stop - item_at), to);
-    at = stop;
+    p.lo = max(unit0 + first, from);
+    p.hi = min(unit0 + first + count, to);
+    at += count;
+    first += count;
+    if (count == rest) {
+      first = 0;
+      if (++tile == tiles) {
+        tile = 0;
+        if (++h == a.c.H) {
+          h = 0;
+          ++b;
+          while (at < end && before[b + 1] <= at) ++b;
+        }
+      }
+    }
     return true;
   }
 };
@@ -147,16 +198,23 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Four codes as f16 numbers: 0x6400 + u is 1024 + u, less 1152
+// Four codes as f16 numbers, 2^-24 of their values
 __device__ __forceinline__ void decode(uint32_t w, uint32_t& b0, uint32_t& b1) {
-  const uint32_t lo = __byte_perm(w, 0x64646464u, 0x4140), hi = __byte_perm(w, 0x64646464u, 0x4342), off = 0x64806480u;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(b0) : "r"(lo), "r"(off));
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(b1) : "r"(hi), "r"(off));
+  b0 = __byte_perm(w, 0u, 0x4140);
+  b1 = __byte_perm(w, 0u, 0x4342);
 }
+constexpr uint32_t kMinus128 = 0x80808080u;              // two of -128 in that form
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void load4(uint32_t (&w)[4], const uint8_t* p) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  w[0] = v.x;
+  w[1] = v.y;
+  w[2] = v.z;
+  w[3] = v.w;
 }
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
@@ -166,9 +224,15 @@ __device__ __forceinline__ float quad_sum(float x) {
   x += __shfl_xor_sync(0xffffffffu, x, 1);
   return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
-               "r"(tc5::smem_u32(bar))
+// Codes are read once a call: they are the first to leave L2, where tables, queries and instructions are wanted again
+__device__ __forceinline__ uint64_t read_once() {
+  uint64_t policy;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(tc5::smem_u32(bar)), "l"(policy)
                : "memory");
 }
 // Exponent of a power of two (NaN for NaN)
@@ -181,35 +245,58 @@ __device__ __forceinline__ float log2_of_scale(float s) {
 template <int D>
 struct Rows {
   uint32_t q[D / 16][4];
-  float factor[2];      // of lane rows r and r + 8: takes a product of f16 queries and codes to x / key scale
+  float factor[2];      // of lane rows r and r + 8: takes a product of f16 queries and code numbers to 2^-24 x / key scale
+  float off[2];         // what the codes' offset adds to such a product
   int pos[2];           // their positions; -1: no row
   float m[2], l[2];
-  float o[D / 8][4];
+  float o[D / 8][4];    // with 128 times the sum of probabilities still in it, whose negative `off_o` is
+  float off_o[4];
 
   __device__ __forceinline__ void clear() {
     m[0] = m[1] = -CUDART_INF_F;
     l[0] = l[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    off_o[0] = off_o[1] = off_o[2] = off_o[3] = 0.f;
+  }
+  __device__ __forceinline__ void settle() {             // takes the offset out of the outputs
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      float2* x = reinterpret_cast<float2*>(o[i]);
+      x[0] = add2(x[0], make_float2(off_o[0], off_o[1]));
+      x[1] = add2(x[1], make_float2(off_o[2], off_o[3]));
+    }
+    off_o[0] = off_o[1] = off_o[2] = off_o[3] = 0.f;
   }
 
-  // Row r of the item is query token r / G, head r % G of the group
-  __device__ __forceinline__ void load(const AttnParams& p, const Piece& it, int row0) {
+  // Row r of the item is query token r / G, head r % G of the group.  Asked for first, taken up when the copies are under way: behind them they
+  // would wait for 30 MB (7000 cycles).
+  struct Raw {
+    uint4 v[2][D / 64][2];
+  };
+  __device__ __forceinline__ void ask(Raw& raw, const AttnParams& p, const Piece& it, int row0) {
     const int lane = threadIdx.x & 31, r = lane & 3;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int row = row0 + (lane >> 2) + 8 * i, t = row / p.G;
+      const int row = row0 + (lane >> 2) + 8 * i, t = token_of(p, row);
       const bool there = t < it.n;
       pos[i] = there ? it.past + t : -1;
-      uint4 raw[D / 64][2];
-      unsigned top = 0;
       const bf16* src = p.q + static_cast<long>(it.q0 + t) * p.ldq + static_cast<long>(it.h * p.G + row - t * p.G) * D + r * 16;
 #pragma unroll
       for (int h = 0; h < D / 64; ++h)
 #pragma unroll
+        for (int k = 0; k < 2; ++k) raw.v[i][h][k] = there ? *reinterpret_cast<const uint4*>(src + h * 64 + k * 8) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void take(const Raw& raw, float softmax_scale) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      unsigned top = 0;
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h)
+#pragma unroll
         for (int k = 0; k < 2; ++k) {
-          raw[h][k] = there ? *reinterpret_cast<const uint4*>(src + h * 64 + k * 8) : make_uint4(0, 0, 0, 0);
-          const uint32_t w[4] = {raw[h][k].x, raw[h][k].y, raw[h][k].z, raw[h][k].w};
+          const uint32_t w[4] = {raw.v[i][h][k].x, raw.v[i][h][k].y, raw.v[i][h][k].z, raw.v[i][h][k].w};
 #pragma unroll
           for (int y = 0; y < 4; ++y) top = max(top, max(w[y] & 0x7fffu, (w[y] >> 16) & 0x7fffu));
         }
@@ -217,19 +304,22 @@ struct Rows {
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = static_cast<int>(top >> 7);                        // the largest magnitude is 2^(e - 127) at least
       const int up = min(140 - e, 126);
-      const float f = __int_as_float((up + 127) << 23);
-      factor[i] = e == 255 ? CUDART_NAN_F : __int_as_float((127 - up) << 23) * p.scale;
+      const float f = softmax_scale < 0.f ? -__int_as_float((up + 127) << 23) : __int_as_float((up + 127) << 23);
+      factor[i] = e == 255 ? CUDART_NAN_F : __int_as_float((127 - up) << 23) * fabsf(softmax_scale);
+      float sum = 0.f;
 #pragma unroll
       for (int h = 0; h < D / 64; ++h)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint32_t w[4] = {raw[h][k].x, raw[h][k].y, raw[h][k].z, raw[h][k].w};
+          const uint32_t w[4] = {raw.v[i][h][k].x, raw.v[i][h][k].y, raw.v[i][h][k].z, raw.v[i][h][k].w};
 #pragma unroll
           for (int y = 0; y < 4; ++y) {                                // columns 16 r + 8 k + 2 y, + 1 of this half
-            const uint32_t v = pack_half(__int_as_float(w[y] << 16) * f, __int_as_float(w[y] & 0xffff0000u) * f);
-            q[h * 4 + k * 2 + (y >> 1)][i + 2 * (y & 1)] = v;
+            const float a = __int_as_float(w[y] << 16) * f, b = __int_as_float(w[y] & 0xffff0000u) * f;
+            sum += a + b;
+            q[h * 4 + k * 2 + (y >> 1)][i + 2 * (y & 1)] = pack_half(a, b);
           }
         }
+      off[i] = quad_sum(sum) * 0x1p-17f;
     }
   }
 };
@@ -240,46 +330,63 @@ __device__ __forceinline__ void scores(const Rows<D>& w, const uint8_t* keys, fl
   const int lane = threadIdx.x & 31, c = lane >> 2, r = lane & 3;
   const uint8_t* base = keys + (c >> 1) * S::kPitch + (c & 1) * 64 + r * 16;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+  for (int j = 0; j < 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+  for (int g = 0; g < 8; g += 4)                                       // four tiles at a time: their products do not wait for one another
 #pragma unroll
     for (int h = 0; h < D / 64; ++h) {
-      const uint4 k = *reinterpret_cast<const uint4*>(base + (j * (D / 64) + h) * 128);
-      const uint32_t words[4] = {k.x, k.y, k.z, k.w};
+      uint32_t words[4][4];
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        uint32_t b0, b1;
-        decode(words[y], b0, b1);
-        mma(s[j], w.q[h * 4 + y], b0, b1);
+      for (int j = 0; j < 4; ++j) load4(words[j], base + ((g + j) * (D / 64) + h) * 128);
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t b0, b1;
+          decode(words[j][y], b0, b1);
+          mma(s[g + j], w.q[h * 4 + y], b0, b1);
+        }
+    }
+}
+
+// Scores to probabilities, in f16 pairs, with the running maximum and sum.  masked: some key of the unit is not seen by some row; such scores become
+// -inf, before x = a s + c with a > 0.
+template <int D>
+__device__ __forceinline__ void softmax(Rows<D>& w, float (&s)[8][4], uint32_t (&pr)[8][2], float2 scale, bool masked, int key0, int window) {
+  const bool there = scale.x != -1.f;                                  // else a sub-block without a page
+  const float ev = there ? log2_of_scale(scale.y) : 0.f, sk = there ? scale.x * 0x1p24f : 0.f;
+  float a[2], c[2], top[2], ref[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    a[i] = w.factor[i] * sk;
+    a[i] = a[i] == 0.f ? 0x1p-126f : a[i];
+    c[i] = fmaf(-w.off[i], a[i], ev);
+    top[i] = -CUDART_INF_F;
+  }
+  if (masked) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // keys 2j + e of the lane's sub-block with from < 2j + e <= to
+      const int to = there ? w.pos[i] - key0 : -1, from = window > 0 ? w.pos[i] - window - key0 : -1;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (2 * j + e > to || 2 * j + e <= from) s[j][2 * i + e] = -CUDART_INF_F;
+      if (to < 0 || from >= 15 || from >= to) {                        // a row that sees nothing of a page does not see that its scale is NaN
+        a[i] = 1.f;
+        c[i] = 0.f;
       }
     }
   }
-}
-
-// Scores to probabilities, in f16 pairs, with the running maximum and sum.  MASKED: some key of the unit is not seen by some row.
-template <int D, bool MASKED>
-__device__ __forceinline__ void softmax(Rows<D>& w, float (&s)[8][4], uint32_t (&pr)[8][2], float2 scale, int key0, int window) {
-  const bool there = scale.x >= 0.f || scale.x != scale.x;             // a sub-block without a page has -1
-  const float ev = there ? log2_of_scale(scale.y) : 0.f;
-  const float a[2] = {there ? w.factor[0] * scale.x : 0.f, there ? w.factor[1] * scale.x : 0.f};
-  float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
   for (int j = 0; j < 8; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float x = fmaf(s[j][i], a[i >> 1], ev);
-      if (MASKED) {
-        const int key = key0 + 2 * j + (i & 1), pos = w.pos[i >> 1];
-        if (!there || key > pos || (window > 0 && key <= pos - window)) x = -CUDART_INF_F;
-      }
-      s[j][i] = x;
-      top[i >> 1] = fmaxf(top[i >> 1], x);
-    }
-  float ref[2];
+    for (int i = 0; i < 4; ++i) top[i >> 1] = fmaxf(top[i >> 1], s[j][i]);
   bool moved = false;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float m = fmaxf(w.m[i], quad_max(top[i]));
+    const float m = fmaxf(w.m[i], quad_max(fmaf(top[i], a[i], c[i])));
     moved |= m != w.m[i];
     ref[i] = m == -CUDART_INF_F ? 0.f : m;
     top[i] = m;
@@ -290,27 +397,32 @@ __device__ __forceinline__ void softmax(Rows<D>& w, float (&s)[8][4], uint32_t (
       const float f = ex2(w.m[i] - ref[i]);
       w.m[i] = top[i];
       w.l[i] *= f;
+      w.off_o[2 * i] *= f;
+      w.off_o[2 * i + 1] *= f;
 #pragma unroll
       for (int d = 0; d < D / 8; ++d) {
-        w.o[d][2 * i] *= f;
-        w.o[d][2 * i + 1] *= f;
+        float2* o = reinterpret_cast<float2*>(w.o[d]);
+        o[i] = mul2(o[i], make_float2(f, f));
       }
     }
   }
-  float sum[2] = {0.f, 0.f};
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 8; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[j][i] = ex2(s[j][i] - ref[i >> 1]);
-      sum[i >> 1] += s[j][i];
+    for (int i = 0; i < 2; ++i) {
+      const float b = c[i] - ref[i];
+      const float2 x = fma2(make_float2(s[j][2 * i], s[j][2 * i + 1]), make_float2(a[i], a[i]), make_float2(b, b));
+      const float2 e = make_float2(ex2(x.x), ex2(x.y));
+      sum[i] = add2(sum[i], e);
+      pr[j][i] = pack_half(e.x, e.y);
     }
-    pr[j][0] = pack_half(s[j][0], s[j][1]);
-    pr[j][1] = pack_half(s[j][2], s[j][3]);
+  const float out = ex2(-ev);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float t = sum[i].x + sum[i].y;
+    w.l[i] += t == 0.f ? 0.f : t * out;
   }
-  const float out = ex2(-ev);                                          // NaN in a page of which a row sees nothing
-  w.l[0] += sum[0] == 0.f ? 0.f : sum[0] * out;
-  w.l[1] += sum[1] == 0.f ? 0.f : sum[1] * out;
 }
 
 template <int D, class S>
@@ -318,25 +430,35 @@ __device__ __forceinline__ void accumulate(Rows<D>& w, const uint8_t* values, co
   const int lane = threadIdx.x & 31;
   const uint8_t* base = values + (lane & 3) * S::kPitch + (lane >> 2) * 16;
 #pragma unroll
-  for (int d = 0; d < D / 8; ++d) {
-    const uint4 v = *reinterpret_cast<const uint4*>(base + d * 128);
-    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+  for (int y = 0; y < 4; ++y) {
+    const uint32_t a[4] = {pr[2 * y][0], pr[2 * y][1], pr[2 * y + 1][0], pr[2 * y + 1][1]};
+    mma(w.off_o, a, kMinus128, kMinus128);
+  }
+#pragma unroll
+  for (int g = 0; g < D / 8; g += 4) {
+    uint32_t words[4][4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) load4(words[d], base + (g + d) * 128);
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      uint32_t b0, b1;
-      decode(words[y], b0, b1);
       const uint32_t a[4] = {pr[2 * y][0], pr[2 * y][1], pr[2 * y + 1][0], pr[2 * y + 1][1]};
-      mma(w.o[d], a, b0, b1);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        uint32_t b0, b1;
+        decode(words[d][y], b0, b1);
+        mma(w.o[g + d], a, b0, b1);
+      }
     }
   }
 }
 
 // Where row r of an item goes; nullptr: there is no such row
 __device__ __forceinline__ bf16* row_of(const AttnParams& p, int n, int q0, int h, int row, int D) {
-  const int t = row / p.G;
+  const int t = token_of(p, row);
   return t < n ? p.o + (static_cast<long>(q0 + t) * p.Hq + h * p.G + row - t * p.G) * D : nullptr;
 }
-__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+// What takes sums of probabilities and code numbers to the output
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 0x1p24f / l; }
 
 template <int D, int MT>
 __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_constant__ AttnParams p) {
@@ -359,7 +481,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
     long long x = 0;
     if (b < B) {
       const Request r = request_of(p, b);
-      x = static_cast<long long>(r.units) * p.c.H * ((r.n * p.G + S::kRows - 1) / S::kRows);
+      sm.request[b] = r;
+      x = static_cast<long long>(r.units(p.window)) * p.c.H * ((r.n * p.G + S::kRows - 1) / S::kRows);
     }
     const long long mine = x;
     for (int d = 1; d < 32; d <<= 1) {
@@ -381,58 +504,59 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
 
   // ---- this worker's range
   const long long workers = static_cast<long long>(gridDim.x) * S::kGroups, each = max((total + workers - 1) / workers, 1ll);
+  const long long begin = min((static_cast<long long>(blockIdx.x) * S::kGroups + grp) * each, total);
   Cursor<S::kRows> use, get;
-  use.at = min((static_cast<long long>(blockIdx.x) * S::kGroups + grp) * each, total);
-  use.end = min(use.at + each, total);
-  int lo = 0, hi = B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (sm.before[mid] <= use.at) lo = mid; else hi = mid;
-  }
-  use.b = lo;
+  use.init(p, sm.before, sm.request, begin, min(begin + each, total));
   get = use;
 
   // ---- the producer's side: tile t of the range is the keys (even) or values (odd) of its unit t / 2
   uint8_t* ring = sm.ring[grp];
   int get_unit = 0, get_stop = 0;                                      // of the piece that `get` is in
-  int page = -1, page_next = -1, blk = 0, blk_next = 0, head = 0, head_next = 0;
-  bool have = false, have_next = false;
-  // Looks up the pages of the unit after the next: one sub-block per lane, four of them
+  struct Where {
+    int page, blk, head;
+    bool have;
+  };
+  Where now{-1, 0, 0, false}, next = now, after = now;
+  // Looks up the pages of the unit two ahead: one sub-block per lane, four of them
   auto look = [&]() {
-    page = page_next;
-    blk = blk_next;
-    head = head_next;
-    have = have_next;
-    have_next = false;
+    now = next;
+    next = after;
+    after.have = false;
     while (get_unit >= get_stop) {
-      if (!get.next_piece(p, sm.before)) return;
+      if (!get.next_piece(p, sm.before, sm.request)) return;
       get_unit = get.p.lo;
       get_stop = get.p.hi;
     }
-    have_next = true;
-    blk_next = get_unit * 4 + (lane & 3);
-    head_next = get.p.h;
-    page_next = blk_next * 16 < get.p.cap ? page_of(p.s, p.c, get.p.b, static_cast<long>(blk_next) * 16) : -1;
+    after.have = true;
+    after.blk = get_unit * 4 + (lane & 3);
+    after.head = get.p.h;
+    // (no test of the entry here: that would wait for it)
+    after.page = after.blk * 16 < get.p.cap ? p.s.table[static_cast<long>(get.p.b) * p.s.W + (after.blk >> (p.c.shift - 4))] : -1;
     ++get_unit;
   };
-  uint32_t issued = 0;
+  const uint64_t policy = read_once();
+  int put = 0;                                                         // the slot of the next tile
+  uint32_t put_round = 0;
+  bool values = false;
   auto issue = [&](bool& ok) {                                         // the next tile, if there is one
-    const bool values = issued & 1;
     if (!values) look();
-    if (!have) return;
-    const uint32_t slot = issued % S::kSlots, round = issued / S::kSlots;
-    if (MT > 1 && round > 0)
-      ok = ok && tc5::mbar_wait_warp(&sm.empty[grp][slot], (round - 1) & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_EMPTY);
+    if (!now.have) return;
+    const int slot = put;
+    if (MT > 1 && put_round > 0)
+      ok = ok && tc5::mbar_wait_warp(&sm.empty[grp][slot], (put_round - 1) & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_EMPTY);
     if (!ok) return;
-    ++issued;
+    if (++put == S::kSlots) {
+      put = 0;
+      ++put_round;
+    }
     uint64_t* bar = &sm.full[grp][slot];
-    const bool there = page >= 0;
+    const bool there = now.page >= 0 && now.page < p.c.pages;
     const unsigned mask = __ballot_sync(0xffffffffu, there) & 0xf;
-    const long ph = static_cast<long>(there ? page : 0) * p.c.H + head;
+    const long ph = static_cast<long>(there ? now.page : 0) * p.c.H + now.head;
     if (lane < 4) {
       if (there) {
-        const long off = ((ph << (p.c.shift - 4)) + (blk & ((1 << (p.c.shift - 4)) - 1))) * S::kSub;
-        bulk_load(tc5::smem_u32(ring + slot * S::kSlot + lane * S::kPitch), (values ? p.c.v : p.c.k) + off, S::kSub, bar);
+        const long off = ((ph << (p.c.shift - 4)) + (now.blk & ((1 << (p.c.shift - 4)) - 1))) * S::kSub;
+        bulk_load(tc5::smem_u32(ring + slot * S::kSlot + lane * S::kPitch), (values ? p.c.v : p.c.k) + off, S::kSub, bar, policy);
       }
       if (!values && there) {
         asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(tc5::smem_u32(&sm.scale[grp][slot][lane])), "l"(p.c.scale + ph * 2) : "memory");
@@ -443,163 +567,211 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
       }
       if (lane == 0) tc5::mbar_expect_tx(bar, __popc(mask) * S::kSub);
     }
+    values = !values;
   };
   bool ok = true;
-  if (mt == 0) {
-    look();                                                            // the first unit's pages are the "next" ones now
-    for (int i = 0; i < S::kSlots; ++i) issue(ok);
-  }
 
   // ---- the consumer's side
   Rows<D> w;
-  uint32_t tile = 0;
+  typename Rows<D>::Raw raw;
+  int slot = 0;                                                        // of the next tile, and how often the ring has gone round
+  uint32_t round = 0;
   Left left{};
   left.some = use.at < use.end;
-  float* ring_f = reinterpret_cast<float*>(ring);
-  while (ok && use.next_piece(p, sm.before)) {
-    const Piece& it = use.p;
-    const int row0 = it.row0 + mt * 16;
-    w.load(p, it, row0);
-    w.clear();
-    // positions of the warp's first and last row
-    const int rows = it.n * p.G, p0 = row0 < rows ? it.past + row0 / p.G : -1, p1 = row0 < rows ? it.past + min(row0 + 15, rows - 1) / p.G : -1;
-    for (int u = it.lo; u < it.hi && ok; ++u) {
-      const int key0 = u * 64;
-      const bool seen = key0 <= p1 && (p.window == 0 || key0 + 63 > p0 - p.window);
-      uint32_t slot = tile % S::kSlots;
-      ok = tc5::mbar_wait_warp(&sm.full[grp][slot], (tile / S::kSlots) & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_FULL);
-      if (!ok) break;
-      uint32_t pr[8][2];
-      if (seen) {
+  Piece it{};
+  bool held = false;                                                   // whether there is a piece whose sums are in w
+  const int r = lane >> 2, col = (lane & 3) * 2;
+  uint32_t pr[8][2];
+  int u2 = 0, u2_end = 0, p0 = -1, p1 = -1, ahead = S::kSlots + 1, row0 = 0;
+  bool full = false, start = true, fresh = false;
+  // One copy of the code at each place: 99 KB of instructions, with two, cost 10000 cycles a call in first fetches.  A turn issues a tile and takes one
+  // up; keys and values of a unit take turns.  The first turn asks for queries, the next only issue (two of them only look up pages), so that a
+  // tile is issued when the one that was in its place has been taken up.
+#pragma unroll 1
+  for (;;) {
+    if (mt == 0 && !start) {
+      issue(ok);
+      if (ahead > 0) {
+        --ahead;
+        continue;
+      }
+    }
+    while (u2 >= u2_end) {
+      const long long piece_end = use.at;
+      const bool more = use.next_piece(p, sm.before, sm.request);
+      if (more) w.ask(raw, p, use.p, use.p.row0 + mt * 16);            // arrives while the sums before are stored
+      if (held) {
+        w.settle();
+        w.l[0] = quad_sum(w.l[0]);
+        w.l[1] = quad_sum(w.l[1]);
+        if (!it.began && !it.open) {                                     // the whole item: its rows are done
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            bf16* out = row_of(p, it.n, it.q0, it.h, it.row0 + mt * 16 + r + 8 * i, D);
+            if (out) {
+              const float f = inverse(w.l[i]);
+#pragma unroll
+              for (int d = 0; d < D / 8; ++d)
+                *reinterpret_cast<__nv_bfloat162*>(out + d * 8 + col) = __floats2bfloat162_rn(w.o[d][2 * i] * f, w.o[d][2 * i + 1] * f);
+            }
+          }
+        } else {
+          const bool is_head = it.began && !it.open && piece_end < use.end;      // more pieces follow
+          float* dst = is_head ? p.head + (static_cast<long>(blockIdx.x) * S::kGroups + grp) * S::kRows * D : reinterpret_cast<float*>(ring);
+          int* item = is_head ? left.head_item : left.tail_item;
+          item[0] = it.b;
+          item[1] = it.h;
+          item[2] = it.row0;
+          if (is_head) {
+            left.head = 1;
+          } else {
+            left.tail = 1;
+            left.began = it.began;
+            left.open = it.open;
+            left.tail_end = it.item_end;
+            // the sums go where the ring is: every warp of the worker has let go of its last tiles
+            if (MT > 1)
+              for (int i = 0; i < S::kSlots; ++i) {                      // a slot's last round: this one before `slot`, else the one before it
+                const uint32_t done = round + (i < slot);
+                if (done > 0) ok = ok && tc5::mbar_wait_warp(&sm.empty[grp][i], (done - 1) & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_EMPTY);
+              }
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int row = mt * 16 + r + 8 * i;
+            if ((lane & 3) == 0) sm.ml[grp][is_head ? 0 : 1][row] = make_float2(w.m[i], w.l[i]);
+#pragma unroll
+            for (int d = 0; d < D / 8; ++d)
+              *reinterpret_cast<float2*>(dst + row * D + d * 8 + col) = make_float2(w.o[d][2 * i], w.o[d][2 * i + 1]);
+          }
+        }
+      }
+      held = more;
+      if (!more) break;
+      it = use.p;
+      row0 = it.row0 + mt * 16;
+      fresh = true;
+      w.clear();
+      // positions of the warp's first and last row
+      const int rows = it.n * p.G;
+      p0 = row0 < rows ? it.past + token_of(p, row0) : -1;
+      p1 = row0 < rows ? it.past + token_of(p, min(row0 + 15, rows - 1)) : -1;
+      full = row0 + 15 < rows;
+      u2 = 2 * it.lo;
+      u2_end = 2 * it.hi;
+    }
+    if (start) {
+      start = false;
+      continue;
+    }
+    ok = ok && held && tc5::mbar_wait_warp(&sm.full[grp][slot], round & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_FULL);
+    if (!ok) break;
+    if (fresh) {
+      w.take(raw, p.scale);
+      fresh = false;
+    }
+    const int key0 = (u2 >> 1) * 64;
+    if (key0 <= p1 && (p.window == 0 || key0 + 63 > p0 - p.window)) {
+      if (u2 & 1) {
+        accumulate<D, S>(w, ring + slot * S::kSlot, pr);
+        if ((u2 & 7) == 7) w.settle();
+      } else {
         const float2 scale = sm.scale[grp][slot][lane & 3];
         float s[8][4];
         scores<D, S>(w, ring + slot * S::kSlot, s);
-        const bool whole = key0 + 63 <= p0 && (p.window == 0 || key0 > p1 - p.window) && row0 + 15 < rows;
-        if (whole && !__any_sync(0xffffffffu, scale.x == -1.f))
-          softmax<D, false>(w, s, pr, scale, 0, 0);
-        else
-          softmax<D, true>(w, s, pr, scale, key0 + 16 * (lane & 3), p.window);
-      }
-      __syncwarp();
-      if (MT > 1 && lane == 0) tc5::mbar_arrive(&sm.empty[grp][slot]);
-      ++tile;
-      if (mt == 0) issue(ok);
-      slot = tile % S::kSlots;
-      ok = ok && tc5::mbar_wait_warp(&sm.full[grp][slot], (tile / S::kSlots) & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_FULL);
-      if (!ok) break;
-      if (seen) accumulate<D, S>(w, ring + slot * S::kSlot, pr);
-      __syncwarp();
-      if (MT > 1 && lane == 0) tc5::mbar_arrive(&sm.empty[grp][slot]);
-      ++tile;
-      if (mt == 0) issue(ok);
-    }
-    if (!ok) break;
-    w.l[0] = quad_sum(w.l[0]);
-    w.l[1] = quad_sum(w.l[1]);
-    const int r = lane >> 2, col = (lane & 3) * 2;
-    if (!it.began && !it.open) {                                       // the whole item: its rows are done
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        bf16* out = row_of(p, it.n, it.q0, it.h, row0 + r + 8 * i, D);
-        if (out) {
-          const float f = inverse(w.l[i]);
-#pragma unroll
-          for (int d = 0; d < D / 8; ++d)
-            *reinterpret_cast<__nv_bfloat162*>(out + d * 8 + col) = __floats2bfloat162_rn(w.o[d][2 * i] * f, w.o[d][2 * i + 1] * f);
-        }
-      }
-    } else {
-      const bool is_head = it.began && !it.open && use.at < use.end;   // more pieces follow
-      float* dst = is_head ? p.head + (static_cast<long>(blockIdx.x) * S::kGroups + grp) * S::kRows * D : ring_f;
-      int* item = is_head ? left.head_item : left.tail_item;
-      item[0] = it.b;
-      item[1] = it.h;
-      item[2] = it.row0;
-      if (is_head) {
-        left.head = 1;
-      } else {
-        left.tail = 1;
-        left.began = it.began;
-        left.open = it.open;
-        left.tail_last = static_cast<int>(((it.item_end - 1) / each) / S::kGroups);
-        // the sums go where the ring is: every warp of the worker has let go of its last tiles
-        if (MT > 1)
-          for (uint32_t t = tile > S::kSlots ? tile - S::kSlots : 0; t < tile; ++t)
-            ok = ok && tc5::mbar_wait_warp(&sm.empty[grp][t % S::kSlots], (t / S::kSlots) & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_EMPTY);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = mt * 16 + r + 8 * i;
-        if ((lane & 3) == 0) sm.ml[grp][is_head ? 0 : 1][row] = make_float2(w.m[i], w.l[i]);
-#pragma unroll
-        for (int d = 0; d < D / 8; ++d)
-          *reinterpret_cast<float2*>(dst + row * D + d * 8 + col) = make_float2(w.o[d][2 * i], w.o[d][2 * i + 1]);
+        const bool whole = full && key0 + 63 <= p0 && (p.window == 0 || key0 > p1 - p.window);
+        softmax<D>(w, s, pr, scale, !whole || __any_sync(0xffffffffu, scale.x == -1.f), key0 + 16 * (lane & 3), p.window);
       }
     }
+    __syncwarp();
+    if (MT > 1 && lane == 0) tc5::mbar_arrive(&sm.empty[grp][slot]);
+    if (++slot == S::kSlots) {
+      slot = 0;
+      ++round;
+    }
+    ++u2;
   }
-  if (!ok && mt == 0)
+  if (sm.abort_flag && mt == 0)
     for (int i = 0; i < S::kSlots; ++i) tc5::mbar_drain(&sm.full[grp][i]);
   if (mt == 0 && lane == 0) sm.left[grp] = left;
   __syncthreads();
   if (sm.abort_flag) {
-    if (tid == 0) p.join[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (tid == 0) p.join[blockIdx.x].any = 0;
     return;
   }
 
   // ---- parts of one item in several workers meet; those of an item that goes beyond the CTA are left for the join
-  int4 join = make_int4(0, 0, 0, 0);
-  for (int g0 = 0; g0 < S::kGroups; ++g0)
-    for (int side = 0; side < 2; ++side) {                             // a chain begins with the first worker's head, or with a last part
-      const Left& a = sm.left[g0];
-      const bool begins = side == 0 ? g0 == 0 && a.head : a.tail && (g0 == 0 || !a.began);
-      if (!begins) continue;
-      const int* item = side == 0 ? a.head_item : a.tail_item;
-      const bool began = side == 0 || a.began;
-      int g1 = g0;
-      bool open = side == 1 && a.open;
-      unsigned heads = side == 0 ? 1u << g0 : 0u;                      // which workers' contributions are heads
-      while (open && g1 + 1 < S::kGroups && sm.left[g1 + 1].some) {
-        const Left& c = sm.left[++g1];
-        if (c.head) heads |= 1u << g1;
-        open = !c.head && c.open;
-      }
-      const Request rq = request_of(p, item[0]);
-      const bool done = !began && !open;
-      for (int e = tid; e < S::kRows * (D / 4); e += kThreads) {
-        const int row = e / (D / 4), d = (e % (D / 4)) * 4;
-        float m = -CUDART_INF_F;
-        for (int g = g0; g <= g1; ++g) m = fmaxf(m, sm.ml[g][heads >> g & 1 ? 0 : 1][row].x);
-        const float ref = m == -CUDART_INF_F ? 0.f : m;
-        float l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int g = g0; g <= g1; ++g) {
-          const bool is_head = heads >> g & 1;
-          const float2 ml = sm.ml[g][is_head ? 0 : 1][row];
-          const float* src = is_head ? p.head + (static_cast<long>(blockIdx.x) * S::kGroups + g) * S::kRows * D : reinterpret_cast<float*>(sm.ring[g]);
-          const float4 x = *reinterpret_cast<const float4*>(src + row * D + d);
-          const float f = ex2(ml.x - ref);
-          l = fmaf(ml.y, f, l);
-          o.x = fmaf(x.x, f, o.x);
-          o.y = fmaf(x.y, f, o.y);
-          o.z = fmaf(x.z, f, o.z);
-          o.w = fmaf(x.w, f, o.w);
+  const Left mine = sm.left[lane < S::kGroups ? lane : 0];
+  const bool is = lane < S::kGroups;
+  const unsigned some = __ballot_sync(0xffffffffu, is && mine.some), heads = __ballot_sync(0xffffffffu, is && mine.head);
+  const unsigned tails = __ballot_sync(0xffffffffu, is && mine.tail), began = __ballot_sync(0xffffffffu, is && mine.tail && mine.began);
+  const unsigned opens = __ballot_sync(0xffffffffu, is && mine.tail && mine.open);
+  // Chains of contributions to one item: lane g looks at the one that worker g's last part begins (it begins its item, or is the first worker's), lane
+  // kGroups at the first worker's head.
+  int g1 = is ? lane : 0;
+  bool open = is && (opens >> lane & 1);
+  const bool chain = is ? (tails >> lane & 1) && (lane == 0 || !(began >> lane & 1)) : lane == S::kGroups && (heads & 1);
+  unsigned from = is ? 0u : 1u;                                        // workers whose contribution is a head
+  while (open && g1 + 1 < S::kGroups && (some >> (g1 + 1) & 1)) {
+    ++g1;
+    from |= heads & (1u << g1);
+    open = !(heads >> g1 & 1) && (opens >> g1 & 1);
+  }
+  const bool before = !is || (began >> lane & 1), goes_on = chain && !before && open;
+  if (warp == 0) {
+    if (goes_on) p.join[blockIdx.x] = Join{1, mine.tail_item[0], mine.tail_item[1], mine.tail_item[2], mine.tail_end, each};
+    if (!__any_sync(0xffffffffu, goes_on) && lane == 0) p.join[blockIdx.x].any = 0;
+  }
+  // A warp takes a row of a chain at a time: lane k has contribution k's maximum and sum, and every lane D / 32 columns
+  constexpr int kCols = D / 32;
+  for (unsigned chains = __ballot_sync(0xffffffffu, chain); chains; chains &= chains - 1) {
+    const int which = __ffs(chains) - 1, first = which < S::kGroups ? which : 0;
+    const int count = __shfl_sync(0xffffffffu, g1, which) - first + 1;
+    const unsigned as_head = __shfl_sync(0xffffffffu, from, which);
+    const bool began_before = __shfl_sync(0xffffffffu, static_cast<int>(before), which), ends = !__shfl_sync(0xffffffffu, static_cast<int>(open), which);
+    const int* item = which < S::kGroups ? sm.left[first].tail_item : sm.left[first].head_item;
+    const Request rq = sm.request[item[0]];
+    const long part = (static_cast<long>(blockIdx.x) * 2 + (began_before ? 0 : 1)) * S::kRows;
+#pragma unroll 1
+    for (int row = warp; row < S::kRows; row += kWarps) {
+      const int g = first + min(lane, count - 1);
+      float2 ml = sm.ml[g][as_head >> g & 1 ? 0 : 1][row];
+      if (lane >= count) ml = make_float2(-CUDART_INF_F, 0.f);
+      float m = ml.x;
+#pragma unroll
+      for (int x = 4; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+      m = __shfl_sync(0xffffffffu, m, 0);
+      const float f = ex2(ml.x - (m == -CUDART_INF_F ? 0.f : m));
+      float l = ml.y * f;
+#pragma unroll
+      for (int x = 4; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+      l = __shfl_sync(0xffffffffu, l, 0);
+      float o[kCols] = {};
+#pragma unroll 4
+      for (int k = 0; k < count; ++k) {
+        const float* src = as_head >> (first + k) & 1 ? p.head + (static_cast<long>(blockIdx.x) * S::kGroups + first + k) * S::kRows * D
+                                                      : reinterpret_cast<float*>(sm.ring[first + k]);
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+        for (int c = 0; c < kCols; c += 2) {
+          const float2 x = *reinterpret_cast<const float2*>(src + row * D + c * 32 + lane * 2);
+          o[c] = fmaf(x.x, fk, o[c]);
+          o[c + 1] = fmaf(x.y, fk, o[c + 1]);
         }
-        if (done) {
-          bf16* out = row_of(p, rq.n, rq.q0, item[1], item[2] + row, D);
-          if (out) {
-            const float f = inverse(l);
-            __nv_bfloat162 y[2] = {__floats2bfloat162_rn(o.x * f, o.y * f), __floats2bfloat162_rn(o.z * f, o.w * f)};
-            *reinterpret_cast<uint2*>(out + d) = *reinterpret_cast<uint2*>(y);
-          }
-        } else {
-          const long slot = static_cast<long>(blockIdx.x) * 2 + (began ? 0 : 1);
-          *reinterpret_cast<float4*>(p.part + (slot * S::kRows + row) * D + d) = o;
-          if (d == 0) p.part_ml[slot * S::kRows + row] = make_float2(m, l);
-        }
       }
-      if (!began && open) join = make_int4(item[0], item[1], item[2], sm.left[g0].tail_last);
+      if (!began_before && ends) {
+        bf16* out = row_of(p, rq.n, rq.q0, item[1], item[2] + row, D);
+        const float n = inverse(l);
+        if (out)
+#pragma unroll
+          for (int c = 0; c < kCols; c += 2) *reinterpret_cast<__nv_bfloat162*>(out + c * 32 + lane * 2) = __floats2bfloat162_rn(o[c] * n, o[c + 1] * n);
+      } else {
+#pragma unroll
+        for (int c = 0; c < kCols; c += 2) *reinterpret_cast<float2*>(p.part + (part + row) * D + c * 32 + lane * 2) = make_float2(o[c], o[c + 1]);
+        if (lane == 0) p.part_ml[part + row] = make_float2(m, l);
+      }
     }
-  if (tid == 0) p.join[blockIdx.x] = join;
+  }
 }
 
 // Parts of items that several CTAs worked on: CTA (c, part) takes some rows of the item that begins in CTA c of the kernel before.
@@ -609,26 +781,31 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_const
   constexpr int kRows = 16 * MT;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x;
-  const int4 j = p.join[c];
-  if (j.w <= c) return;
-  const Request rq = request_of(p, j.x);
+  const Join j = p.join[c];
+  if (!j.any) return;
+  const Request rq = request_of(p, j.b);
+  const int last = static_cast<int>((j.end - 1) / j.each / (kWarps / MT));
   for (int e = blockIdx.y * 128 + threadIdx.x; e < kRows * (D / 4); e += kJoinParts * 128) {
     const int row = e / (D / 4), d = (e % (D / 4)) * 4;
-    bf16* out = row_of(p, rq.n, rq.q0, j.y, j.z + row, D);
+    bf16* out = row_of(p, rq.n, rq.q0, j.h, j.row0 + row, D);
     if (!out) continue;
     float m = -CUDART_INF_F, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int g = c; g <= j.w; ++g) {
-      const long slot = static_cast<long>(g) * 2 + (g == c);
-      const float2 ml = p.part_ml[slot * kRows + row];
-      const float4 x = *reinterpret_cast<const float4*>(p.part + (slot * kRows + row) * D + d);
-      const float mn = fmaxf(m, ml.x), ref = mn == -CUDART_INF_F ? 0.f : mn, f = ex2(m - ref), h = ex2(ml.x - ref);
-      m = mn;
-      l = l * f + ml.y * h;
-      o.x = o.x * f + x.x * h;
-      o.y = o.y * f + x.y * h;
-      o.z = o.z * f + x.z * h;
-      o.w = o.w * f + x.w * h;
+    // two passes of independent loads: CTA c's second part, the first parts of those behind it
+#pragma unroll 8
+    for (int g = c; g <= last; ++g) m = fmaxf(m, p.part_ml[(static_cast<long>(g) * 2 + (g == c)) * kRows + row].x);
+    const float ref = m == -CUDART_INF_F ? 0.f : m;
+#pragma unroll 8
+    for (int g = c; g <= last; ++g) {
+      const long slot = (static_cast<long>(g) * 2 + (g == c)) * kRows + row;
+      const float2 ml = p.part_ml[slot];
+      const float4 x = *reinterpret_cast<const float4*>(p.part + slot * D + d);
+      const float f = ex2(ml.x - ref);
+      l = fmaf(ml.y, f, l);
+      o.x = fmaf(x.x, f, o.x);
+      o.y = fmaf(x.y, f, o.y);
+      o.z = fmaf(x.z, f, o.z);
+      o.w = fmaf(x.w, f, o.w);
     }
     const float f = inverse(l);
     __nv_bfloat162 y[2] = {__floats2bfloat162_rn(o.x * f, o.y * f), __floats2bfloat162_rn(o.z * f, o.w * f)};
@@ -640,8 +817,17 @@ template <int D, int MT>
 cudaError_t run(const AttnParams& p, int grid, cudaStream_t st) {
   constexpr int bytes = sizeof(Smem<D, MT>);
   static_assert(bytes <= 232448, "shared memory of one CTA");
-  cudaError_t e = cudaFuncSetAttribute(cache_attn_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return e;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static std::atomic<unsigned long long> ready{0};                     // devices on which the kernel may have this much shared memory
+  cudaError_t e = cudaSuccess;
+  if (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(cache_attn_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    // the same division of shared memory for the join: an SM changes it only when it is empty
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(cache_attn_join_kernel<D, MT>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return e;
+    if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   cache_attn_kernel<D, MT><<<grid, kThreads, bytes, st>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
@@ -666,7 +852,7 @@ int row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 
 // Floats of scratch that nsa_cache_attention needs
 extern "C" long nsa_cache_attention_scratch(int Hq, int H, int D, int max_new) {
   const long G = H > 0 ? Hq / H : 1, mt = row_tiles(static_cast<int>(G * max_new < 1024 ? G * max_new : 1024)), grid = nsa::sm_count(), rows = 16 * mt;
-  return grid * (kWarps / mt) * rows * D + grid * 2 * rows * (D + 2) + grid * 4;
+  return grid * (kWarps / mt) * rows * D + grid * 2 * rows * (D + 2) + grid * static_cast<long>(sizeof(Join) / 4);
 }
 
 extern "C" int nsa_cache_attention(const void* q, long ldq, const void* kc, const void* vc, const float* scale, const int* table, const int* query_start,
@@ -682,6 +868,7 @@ extern "C" int nsa_cache_attention(const void* q, long ldq, const void* kc, cons
   p.o = static_cast<bf16*>(o);
   p.Hq = Hq;
   p.G = Hq / H;
+  p.per_g = ((1ull << 32) + p.G - 1) / p.G;
   p.window = window;
   p.scale = softmax_scale * 1.4426950408889634f;
   p.status = nsa::status_ptr();
@@ -689,10 +876,10 @@ extern "C" int nsa_cache_attention(const void* q, long ldq, const void* kc, cons
   const int mt = row_tiles(static_cast<int>(most < 1024 ? most : 1024)), grid = nsa::sm_count(), rows = 16 * mt;
   p.part = scratch;
   p.part_ml = reinterpret_cast<float2*>(p.part + static_cast<long>(grid) * 2 * rows * D);
-  p.join = reinterpret_cast<int4*>(p.part_ml + static_cast<long>(grid) * 2 * rows);
+  p.join = reinterpret_cast<Join*>(p.part_ml + static_cast<long>(grid) * 2 * rows);
   p.head = reinterpret_cast<float*>(p.join + grid);
   cudaError_t e = cudaSuccess;
-  for (int b = 0; b < B && e == cudaSuccess; b += kMaxRequests) {      // a launch for each 1024 requests, on the same scratch
+  for (int b = 0; b < B && e == cudaSuccess; b += kMaxRequests) {      // a launch for each 768 requests, on the same scratch
     p.s = CacheStep{table + static_cast<long>(b) * W, query_start + b, lengths + b, B - b < kMaxRequests ? B - b : kMaxRequests, W, N};
     if (D == 128)
       e = mt == 1 ? run<128, 1>(p, grid, st) : mt == 2 ? run<128, 2>(p, grid, st) : mt == 4 ? run<128, 4>(p, grid, st) : run<128, 8>(p, grid, st);

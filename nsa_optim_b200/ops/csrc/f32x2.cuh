@@ -17,3 +17,10 @@ __device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const f
         "l"(reinterpret_cast<const unsigned long long&>(c)));
   return d;
 }
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
+}
