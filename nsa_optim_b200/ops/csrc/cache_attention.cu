@@ -6,7 +6,7 @@
 //  * Work is counted in units of 64 keys, over all requests, KV heads and row tiles, and dealt out evenly to workers (a warp with 16 rows, more
 //    warps on the same keys where a request has more rows): ragged requests cost no more than even ones.  A worker's range may end inside a request;
 //    such parts meet in shared memory at the CTA's end, and across CTAs in cache_attn_join_kernel.
-//  * Each worker has its own ring of key and value tiles that bulk copies fill two tiles ahead: 130 KB in flight per SM, no registers, and no
+//  * Each worker has its own ring of key and value tiles that asynchronous copies fill two tiles ahead: 130 KB in flight per SM, no registers, and no
 //    synchronisation between workers.
 //  * The cache's orders are those of the product's operands.  Of a unit, lane 4c+r of a warp scores token 2j + c%2 of sub-block c/2 in tile j and holds
 //    the probabilities of sub-block r's tokens 2j, 2j+1, so its value operand is 16 neighbouring bytes.
@@ -50,8 +50,8 @@ struct AttnParams {
 };
 
 // The item that begins in a CTA and ends in another, if there is one
-struct Join {
-  int any, b, h, row0;
+struct alignas(16) Join {
+  int any, h, row0, n, q0, pad;
   long long end, each;  // the unit at which it ends, units of a worker
 };
 
@@ -224,17 +224,6 @@ __device__ __forceinline__ float quad_sum(float x) {
   x += __shfl_xor_sync(0xffffffffu, x, 1);
   return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
-// Codes are read once a call: they are the first to leave L2, where tables, queries and instructions are wanted again
-__device__ __forceinline__ uint64_t read_once() {
-  uint64_t policy;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-  return policy;
-}
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(dst), "l"(src),
-               "r"(bytes), "r"(tc5::smem_u32(bar)), "l"(policy)
-               : "memory");
-}
 // Exponent of a power of two (NaN for NaN)
 __device__ __forceinline__ float log2_of_scale(float s) {
   const int e = static_cast<int>(__float_as_uint(s) >> 23) - 127;
@@ -353,7 +342,7 @@ __device__ __forceinline__ void scores(const Rows<D>& w, const uint8_t* keys, fl
 // -inf, before x = a s + c with a > 0.
 template <int D>
 __device__ __forceinline__ void softmax(Rows<D>& w, float (&s)[8][4], uint32_t (&pr)[8][2], float2 scale, bool masked, int key0, int window) {
-  const bool there = scale.x != -1.f;                                  // else a sub-block without a page
+  const bool there = scale.x != 0.f;                                   // else a sub-block without a page
   const float ev = there ? log2_of_scale(scale.y) : 0.f, sk = there ? scale.x * 0x1p24f : 0.f;
   float a[2], c[2], top[2], ref[2];
 #pragma unroll
@@ -471,10 +460,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
   // ---- the units of all requests
   if (tid == 0) sm.abort_flag = 0;
   for (int i = tid; i < S::kGroups * S::kSlots; i += kThreads) {
-    tc5::mbar_init(&sm.full[0][0] + i, 5);
+    tc5::mbar_init(&sm.full[0][0] + i, 32);
     tc5::mbar_init(&sm.empty[0][0] + i, MT);
   }
   tc5::fence_barrier_init();
+  asm volatile("griddepcontrol.wait;" ::: "memory");                   // until here the kernel may run beside the one before it
   long long total = 0;
   for (int base = 0; base < B; base += kThreads) {
     const int b = base + tid;
@@ -534,7 +524,6 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
     after.page = after.blk * 16 < get.p.cap ? p.s.table[static_cast<long>(get.p.b) * p.s.W + (after.blk >> (p.c.shift - 4))] : -1;
     ++get_unit;
   };
-  const uint64_t policy = read_once();
   int put = 0;                                                         // the slot of the next tile
   uint32_t put_round = 0;
   bool values = false;
@@ -549,24 +538,25 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
       put = 0;
       ++put_round;
     }
-    uint64_t* bar = &sm.full[grp][slot];
+    // 16 bytes at a time by all lanes: a 2 KB bulk copy per sub-block took its lane 110 cycles, 520 a tile, in the way of the products
     const bool there = now.page >= 0 && now.page < p.c.pages;
-    const unsigned mask = __ballot_sync(0xffffffffu, there) & 0xf;
     const long ph = static_cast<long>(there ? now.page : 0) * p.c.H + now.head;
-    if (lane < 4) {
-      if (there) {
-        const long off = ((ph << (p.c.shift - 4)) + (now.blk & ((1 << (p.c.shift - 4)) - 1))) * S::kSub;
-        bulk_load(tc5::smem_u32(ring + slot * S::kSlot + lane * S::kPitch), (values ? p.c.v : p.c.k) + off, S::kSub, bar, policy);
-      }
-      if (!values && there) {
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(tc5::smem_u32(&sm.scale[grp][slot][lane])), "l"(p.c.scale + ph * 2) : "memory");
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc5::smem_u32(bar)) : "memory");
-      } else {
-        if (!values) sm.scale[grp][slot][lane] = make_float2(-1.f, 1.f);
-        tc5::mbar_arrive(bar);
-      }
-      if (lane == 0) tc5::mbar_expect_tx(bar, __popc(mask) * S::kSub);
+    const uint8_t* mine = (values ? p.c.v : p.c.k) + ((ph << (p.c.shift - 4)) + (now.blk & ((1 << (p.c.shift - 4)) - 1))) * S::kSub;
+    const unsigned mask = __ballot_sync(0xffffffffu, there);
+    const uint32_t dst = tc5::smem_u32(ring + slot * S::kSlot) + lane * 16;
+#pragma unroll
+    for (int sub = 0; sub < 4; ++sub) {
+      const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), sub)) + lane * 16;
+      if (mask >> sub & 1)
+#pragma unroll
+        for (int k = 0; k < S::kSub / 512; ++k)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + sub * S::kPitch + k * 512), "l"(src + k * 512) : "memory");
     }
+    if (!values && lane < 4)                                           // zeros where there is no page
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(tc5::smem_u32(&sm.scale[grp][slot][lane])), "l"(p.c.scale + ph * 2),
+                   "r"(there ? 8 : 0)
+                   : "memory");
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc5::smem_u32(&sm.full[grp][slot])) : "memory");
     values = !values;
   };
   bool ok = true;
@@ -680,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
         float s[8][4];
         scores<D, S>(w, ring + slot * S::kSlot, s);
         const bool whole = full && key0 + 63 <= p0 && (p.window == 0 || key0 > p1 - p.window);
-        softmax<D>(w, s, pr, scale, !whole || __any_sync(0xffffffffu, scale.x == -1.f), key0 + 16 * (lane & 3), p.window);
+        softmax<D>(w, s, pr, scale, !whole || __any_sync(0xffffffffu, scale.x == 0.f), key0 + 16 * (lane & 3), p.window);
       }
     }
     __syncwarp();
@@ -691,8 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
     }
     ++u2;
   }
-  if (sm.abort_flag && mt == 0)
-    for (int i = 0; i < S::kSlots; ++i) tc5::mbar_drain(&sm.full[grp][i]);
+  asm volatile("cp.async.wait_all;" ::: "memory");
   if (mt == 0 && lane == 0) sm.left[grp] = left;
   __syncthreads();
   if (sm.abort_flag) {
@@ -719,55 +708,61 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
   }
   const bool before = !is || (began >> lane & 1), goes_on = chain && !before && open;
   if (warp == 0) {
-    if (goes_on) p.join[blockIdx.x] = Join{1, mine.tail_item[0], mine.tail_item[1], mine.tail_item[2], mine.tail_end, each};
+    if (goes_on) {
+      const Request rq = sm.request[mine.tail_item[0]];
+      p.join[blockIdx.x] = Join{1, mine.tail_item[1], mine.tail_item[2], rq.n, rq.q0, 0, mine.tail_end, each};
+    }
     if (!__any_sync(0xffffffffu, goes_on) && lane == 0) p.join[blockIdx.x].any = 0;
   }
-  // A warp takes a row of a chain at a time: lane k has contribution k's maximum and sum, and every lane D / 32 columns
+  // A warp takes a row of a chain at a time, a lane D / 32 columns of it, all contributions at once.  Only the last of a chain, which closes it, may be a
+  // head.
   constexpr int kCols = D / 32;
   for (unsigned chains = __ballot_sync(0xffffffffu, chain); chains; chains &= chains - 1) {
-    const int which = __ffs(chains) - 1, first = which < S::kGroups ? which : 0;
-    const int count = __shfl_sync(0xffffffffu, g1, which) - first + 1;
-    const unsigned as_head = __shfl_sync(0xffffffffu, from, which);
+    const int which = __ffs(chains) - 1, first = which < S::kGroups ? which : 0, last = __shfl_sync(0xffffffffu, g1, which);
+    const bool closed = __shfl_sync(0xffffffffu, static_cast<int>(from != 0), which);              // by a head
     const bool began_before = __shfl_sync(0xffffffffu, static_cast<int>(before), which), ends = !__shfl_sync(0xffffffffu, static_cast<int>(open), which);
     const int* item = which < S::kGroups ? sm.left[first].tail_item : sm.left[first].head_item;
     const Request rq = sm.request[item[0]];
+    const int stop = last + !closed;                                   // tails: first .. stop - 1
+    const float* head = p.head + (static_cast<long>(blockIdx.x) * S::kGroups + last) * S::kRows * D;
     const long part = (static_cast<long>(blockIdx.x) * 2 + (began_before ? 0 : 1)) * S::kRows;
-#pragma unroll 1
+#pragma unroll 2
     for (int row = warp; row < S::kRows; row += kWarps) {
-      const int g = first + min(lane, count - 1);
-      float2 ml = sm.ml[g][as_head >> g & 1 ? 0 : 1][row];
-      if (lane >= count) ml = make_float2(-CUDART_INF_F, 0.f);
-      float m = ml.x;
+      float2 x[S::kGroups + 1][kCols / 2], ml[S::kGroups + 1];
+      const int at = row * D + lane * 2;
+      ml[S::kGroups] = closed ? sm.ml[last][0][row] : make_float2(-CUDART_INF_F, 0.f);
 #pragma unroll
-      for (int x = 4; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-      m = __shfl_sync(0xffffffffu, m, 0);
-      const float f = ex2(ml.x - (m == -CUDART_INF_F ? 0.f : m));
-      float l = ml.y * f;
+      for (int c = 0; c < kCols / 2; ++c)
+        x[S::kGroups][c] = closed ? *reinterpret_cast<const float2*>(head + at + c * 64) : make_float2(0.f, 0.f);
 #pragma unroll
-      for (int x = 4; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-      l = __shfl_sync(0xffffffffu, l, 0);
-      float o[kCols] = {};
-#pragma unroll 4
-      for (int k = 0; k < count; ++k) {
-        const float* src = as_head >> (first + k) & 1 ? p.head + (static_cast<long>(blockIdx.x) * S::kGroups + first + k) * S::kRows * D
-                                                      : reinterpret_cast<float*>(sm.ring[first + k]);
-        const float fk = __shfl_sync(0xffffffffu, f, k);
+      for (int g = 0; g < S::kGroups; ++g) {
+        const bool in = g >= first && g < stop;
+        ml[g] = in ? sm.ml[g][1][row] : make_float2(-CUDART_INF_F, 0.f);
 #pragma unroll
-        for (int c = 0; c < kCols; c += 2) {
-          const float2 x = *reinterpret_cast<const float2*>(src + row * D + c * 32 + lane * 2);
-          o[c] = fmaf(x.x, fk, o[c]);
-          o[c + 1] = fmaf(x.y, fk, o[c + 1]);
-        }
+        for (int c = 0; c < kCols / 2; ++c)
+          x[g][c] = in ? *reinterpret_cast<const float2*>(sm.ring[g] + (at + c * 64) * 4) : make_float2(0.f, 0.f);
+      }
+      float m = -CUDART_INF_F, l = 0.f;
+#pragma unroll
+      for (int g = 0; g <= S::kGroups; ++g) m = fmaxf(m, ml[g].x);
+      const float ref = m == -CUDART_INF_F ? 0.f : m;
+      float2 o[kCols / 2] = {};
+#pragma unroll
+      for (int g = 0; g <= S::kGroups; ++g) {
+        const float f = ex2(ml[g].x - ref);
+        l = fmaf(ml[g].y, f, l);
+#pragma unroll
+        for (int c = 0; c < kCols / 2; ++c) o[c] = fma2(x[g][c], make_float2(f, f), o[c]);
       }
       if (!began_before && ends) {
         bf16* out = row_of(p, rq.n, rq.q0, item[1], item[2] + row, D);
         const float n = inverse(l);
         if (out)
 #pragma unroll
-          for (int c = 0; c < kCols; c += 2) *reinterpret_cast<__nv_bfloat162*>(out + c * 32 + lane * 2) = __floats2bfloat162_rn(o[c] * n, o[c + 1] * n);
+          for (int c = 0; c < kCols / 2; ++c) *reinterpret_cast<__nv_bfloat162*>(out + lane * 2 + c * 64) = __floats2bfloat162_rn(o[c].x * n, o[c].y * n);
       } else {
 #pragma unroll
-        for (int c = 0; c < kCols; c += 2) *reinterpret_cast<float2*>(p.part + (part + row) * D + c * 32 + lane * 2) = make_float2(o[c], o[c + 1]);
+        for (int c = 0; c < kCols / 2; ++c) *reinterpret_cast<float2*>(p.part + part * D + at + c * 64) = o[c];
         if (lane == 0) p.part_ml[part + row] = make_float2(m, l);
       }
     }
@@ -779,33 +774,46 @@ constexpr int kJoinParts = 4;
 template <int D, int MT>
 __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_constant__ AttnParams p) {
   constexpr int kRows = 16 * MT;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x;
   const Join j = p.join[c];
   if (!j.any) return;
-  const Request rq = request_of(p, j.b);
   const int last = static_cast<int>((j.end - 1) / j.each / (kWarps / MT));
   for (int e = blockIdx.y * 128 + threadIdx.x; e < kRows * (D / 4); e += kJoinParts * 128) {
     const int row = e / (D / 4), d = (e % (D / 4)) * 4;
-    bf16* out = row_of(p, rq.n, rq.q0, j.h, j.row0 + row, D);
+    bf16* out = row_of(p, j.n, j.q0, j.h, j.row0 + row, D);
     if (!out) continue;
     float m = -CUDART_INF_F, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    // two passes of independent loads: CTA c's second part, the first parts of those behind it
-#pragma unroll 8
-    for (int g = c; g <= last; ++g) m = fmaxf(m, p.part_ml[(static_cast<long>(g) * 2 + (g == c)) * kRows + row].x);
-    const float ref = m == -CUDART_INF_F ? 0.f : m;
-#pragma unroll 8
-    for (int g = c; g <= last; ++g) {
-      const long slot = (static_cast<long>(g) * 2 + (g == c)) * kRows + row;
-      const float2 ml = p.part_ml[slot];
-      const float4 x = *reinterpret_cast<const float4*>(p.part + slot * D + d);
-      const float f = ex2(ml.x - ref);
-      l = fmaf(ml.y, f, l);
-      o.x = fmaf(x.x, f, o.x);
-      o.y = fmaf(x.y, f, o.y);
-      o.z = fmaf(x.z, f, o.z);
-      o.w = fmaf(x.w, f, o.w);
+    for (int g0 = c; g0 <= last; g0 += 8) {                            // CTA c's second part, the first parts of those behind it, eight at once
+      float2 ml[8];
+      float4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int g = min(g0 + i, last);
+        const long slot = (static_cast<long>(g) * 2 + (g == c)) * kRows + row;
+        ml[i] = p.part_ml[slot];
+        x[i] = *reinterpret_cast<const float4*>(p.part + slot * D + d);
+        if (g0 + i > last) ml[i] = make_float2(-CUDART_INF_F, 0.f);
+      }
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
+      const float ref = mn == -CUDART_INF_F ? 0.f : mn, keep = ex2(m - ref);
+      m = mn;
+      l *= keep;
+      o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = ex2(ml[i].x - ref);
+        if (g0 + i > last) continue;
+        l = fmaf(ml[i].y, f, l);
+        o.x = fmaf(x[i].x, f, o.x);
+        o.y = fmaf(x[i].y, f, o.y);
+        o.z = fmaf(x[i].z, f, o.z);
+        o.w = fmaf(x[i].w, f, o.w);
+      }
     }
     const float f = inverse(l);
     __nv_bfloat162 y[2] = {__floats2bfloat162_rn(o.x * f, o.y * f), __floats2bfloat162_rn(o.z * f, o.w * f)};
@@ -828,18 +836,21 @@ cudaError_t run(const AttnParams& p, int grid, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  cache_attn_kernel<D, MT><<<grid, kThreads, bytes, st>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, kJoinParts);
-  cfg.blockDim = 128;
+  cfg.gridDim = grid;
+  cfg.blockDim = kThreads;
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, MT>, p);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3(grid, kJoinParts);
+  cfg.blockDim = 128;
+  cfg.dynamicSmemBytes = 0;
   e = cudaLaunchKernelEx(&cfg, cache_attn_join_kernel<D, MT>, p);
   nsa::count_launch(2);
   return e;
