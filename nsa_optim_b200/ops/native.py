@@ -1260,4 +1260,7 @@ class _TokenLogprobs(torch.autograd.Function):
 
 
 def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
+    if 32 < top_k <= logits.shape[-1]:
+        _fallback("token_logprobs")
+        return torch_impl.token_logprobs(logits, tokens, top_k, ignore_index)
     return torch_impl.TokenLogprobs(*_run(_TokenLogprobs, logits, tokens, top_k, ignore_index))
