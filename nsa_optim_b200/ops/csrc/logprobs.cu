@@ -7,26 +7,34 @@
 // be 2^-24 of the largest logit in log S, is taken out at the end: log2(e) m - R is known to its last bit.
 //
 // The bytes of the logits bound both directions (an exponential takes 72 % of the special-function rate at that speed, the arithmetic 45 % of issue).
-// The k likeliest tokens cost next to nothing in the pass: each thread keeps the maximum of what it saw.  The k-th largest of the maxima of 64 groups of
-// threads is a bound that k logits reach, so only the pieces of threads whose maximum reaches it are looked at again (about k of 256, unless
-// logits are equal).
+// The k likeliest tokens cost next to nothing in the pass: each thread keeps the largest logit of what it saw, the four pieces it was in, and the largest
+// of the other pieces.  The k-th largest of the maxima of 64 pairs of threads is a bound that k logits reach, so only the four pieces of threads whose
+// maximum reaches it are read again (few more than k of 128 threads), and all pieces of a thread where a second four do.  A warp of its own does that,
+// and the row's end, while the others are in the next row.  What it waits for counts: behind 24 MB of copies a load takes 4 us, so that it reads what it
+// needs at once (when it read whole threads' pieces in turns, 4096 x 151936 logits with k = 8 took 413 us, with k = 1 230).
 //
 // Compiled without fast math: the logarithms at a row's end are the exact ones, the exponentials of its elements the hardware's.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <math_constants.h>
 
+#include <atomic>
+
 #include "f32x2.cuh"
 #include "host.cuh"
+#include "tc5.cuh"
 
 namespace {
 namespace cg = cooperative_groups;
 typedef __nv_bfloat16 bf16;
 typedef unsigned long long u64;
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kUnroll = 4;                // 16-byte loads of a thread in flight
+constexpr int kThreads = 128, kWarps = kThreads / 32;        // of the pass over the logits; a warp more for the copies, one for the rows' ends
+constexpr int kCtas = 5;                  // per SM
+constexpr int kUnroll = 4, kHalves = 2;   // 16-byte pieces of a thread at a time; of a chunk
+constexpr int kChunk = kThreads * kUnroll * kHalves, kStages = 2;      // pieces that a bulk copy brings (16 KB); chunks on their way or in use
 constexpr int kTopMax = 32;               // tokens that the selection gives
-constexpr int kBuffer = 1024;             // candidates for them
+constexpr int kBuffer = 512;              // candidates for them
+constexpr int kWidest = 32767 * kThreads * kUnroll * 4;      // columns: halves of chunks are counted in 16 bits
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLow = -1e30f;            // logits below it count as this in the pass: 2^-inf times -inf is no number
 
@@ -65,10 +73,27 @@ template <>
 struct Vec<bf16> {
   static constexpr int kN = 8;
   uint4 w;
+  static __device__ __forceinline__ float top(const Vec (&v)[kUnroll]) {
+    uint4 m = v[0].w;
+#pragma unroll
+    for (int u = 1; u < kUnroll; ++u) m = make_uint4(max2_nan(m.x, v[u].w.x), max2_nan(m.y, v[u].w.y), max2_nan(m.z, v[u].w.z), max2_nan(m.w, v[u].w.w));
+    return Vec{m}.top();
+  }
   __device__ __forceinline__ float top() const {
     const uint32_t m = max2_nan(max2_nan(w.x, w.y), max2_nan(w.z, w.w));
     return max_nan(lower(m), upper(m));
   }
+  __device__ __forceinline__ void exact(float2 (&x)[4]) const {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = make_float2(lower(v[i]), upper(v[i]));
+  }
+  static __device__ __forceinline__ uint32_t two(float2 x) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x.x, x.y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ uint4 pack(const float2 (&x)[4]) { return make_uint4(two(x[0]), two(x[1]), two(x[2]), two(x[3])); }
+  __device__ __forceinline__ void clear() { w = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
   __device__ __forceinline__ void floats(float2 (&x)[4]) const {       // none below kLow
     const uint32_t v[4] = {w.x, w.y, w.z, w.w}, low = 0xf149f149u;     // bf16 of -1e30
 #pragma unroll
@@ -82,7 +107,21 @@ template <>
 struct Vec<float> {
   static constexpr int kN = 4;
   float4 w;
+  static __device__ __forceinline__ float top(const Vec (&v)[kUnroll]) {
+    float m = v[0].top();
+#pragma unroll
+    for (int u = 1; u < kUnroll; ++u) m = max_nan(m, v[u].top());
+    return m;
+  }
   __device__ __forceinline__ float top() const { return max_nan(max_nan(w.x, w.y), max_nan(w.z, w.w)); }
+  __device__ __forceinline__ void exact(float2 (&x)[2]) const {
+    x[0] = make_float2(w.x, w.y);
+    x[1] = make_float2(w.z, w.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float2 (&x)[2]) {
+    return make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x), __float_as_uint(x[1].y));
+  }
+  __device__ __forceinline__ void clear() { w = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F); }
   __device__ __forceinline__ void floats(float2 (&x)[2]) const {
     x[0] = make_float2(max_nan(w.x, kLow), max_nan(w.y, kLow));
     x[1] = make_float2(max_nan(w.z, kLow), max_nan(w.w, kLow));
@@ -101,6 +140,10 @@ __device__ __forceinline__ unsigned ordered(float x) {
   return bits >= 0 ? static_cast<unsigned>(bits) | 0x80000000u : ~static_cast<unsigned>(bits);
 }
 __device__ __forceinline__ u64 rank_of(float x, int i) { return static_cast<u64>(ordered(x)) << 32 | (0xffffffffu - static_cast<unsigned>(i)); }
+__device__ __forceinline__ float logit_of(u64 r) {
+  const unsigned o = static_cast<unsigned>(r >> 32);
+  return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o);
+}
 __device__ __forceinline__ int index_of(u64 r) { return static_cast<int>(0xffffffffu - static_cast<unsigned>(r)); }
 
 // Sums over some logits, of which m is the largest; none yet (or none above kLow) where m is kLow
@@ -123,31 +166,43 @@ struct Sums {
   }
 };
 
-// A CTA's part of a row: columns lo .. hi, as 16-byte pieces, the first and last of which may reach beyond it.  Piece j is thread j % kThreads'.
+// A CTA's part of a row: columns lo .. hi, as 16-byte pieces, the first and last of which may reach beyond it.  Of the whole ones, w0 .. w1, piece w0 + j is
+// thread j % kThreads'; a first one that is not whole is thread 0's, a last one thread 32's.
 template <class T>
 struct Part {
   static constexpr int kN = Vec<T>::kN;
   const T* x;           // column 0
   int lo, hi, base;     // the first piece begins at column base <= lo, which is 16-byte aligned
-  int pieces;
+  int pieces, w0, w1;
   __device__ __forceinline__ Part(const T* row, int l, int h) : x(row), lo(l), hi(h) {
     const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row + lo) % 16 / sizeof(T));
     base = lo - off;
     pieces = hi > lo ? (hi - base + kN - 1) / kN : 0;
+    w0 = off > 0 && pieces > 0 ? 1 : 0;
+    w1 = max((hi - base) / kN, w0);
   }
-  __device__ __forceinline__ bool whole(int j) const { return (j > 0 || base == lo) && base + (j + 1) * kN <= hi; }
+  __device__ __forceinline__ int chunks() const { return (w1 - w0 + kChunk - 1) / kChunk; }
+  __device__ __forceinline__ const T* chunk(int c) const { return x + base + static_cast<long>(w0 + c * kChunk) * kN; }
+  __device__ __forceinline__ int chunk_pieces(int c) const { return min(kChunk, w1 - w0 - c * kChunk); }
+  // The piece of a thread that is not whole, -1: none
+  __device__ __forceinline__ int odd_piece(int t) const { return t == 0 && w0 == 1 ? 0 : t == 32 && w1 < pieces ? w1 : -1; }
   __device__ __forceinline__ float at(int c) const { return c >= lo && c < hi ? value(x, c) : -CUDART_INF_F; }
 };
 
 struct Smem {
-  Sums sums[kWarps], all;
-  float top[kThreads];
-  unsigned group[64], kth;                 // maxima of neighbouring threads; the bound, as `ordered`
-  int count, reach, above;
-  short list[kThreads];                    // threads whose pieces are looked at again
+  // what the pass leaves for a row's end, of two rows in turn
+  Sums sums[2][kWarps];
+  alignas(16) unsigned top[2][kThreads];   // maxima of threads, as `ordered`
+  alignas(16) unsigned other[2][kThreads]; // of the pieces that do not lie with it
+  alignas(8) short where[2][kThreads];     // the chunk half that it lies in; -1: a piece that is not whole
+  uint64_t ready[2], taken[2];
+  // the fifth warp's
+  Sums all;
+  short list[kThreads], rest[kThreads];    // threads of which four pieces, or all, are looked at again
   u64 buffer[kBuffer];
   u64 best[kTopMax];
-  u64 red[kWarps];
+  uint64_t full[kStages], empty[kStages];
+  int abort_flag;
 };
 
 __device__ __forceinline__ void warp_reduce(Sums& s) {                 // lanes share m
@@ -157,19 +212,25 @@ __device__ __forceinline__ void warp_reduce(Sums& s) {                 // lanes 
   }
 }
 
-// The sums of a part and the thread's own maximum
+// The sums of a part and the thread's own maximum.  get: chunks that the CTA has read
 template <class T>
-__device__ __forceinline__ Sums pass(const Part<T>& p, float& top) {
+__device__ __forceinline__ Sums pass(const Part<T>& p, Smem& sm, const uint4* ring, uint32_t& get, bool& ok, float& top, float& other, int& where,
+                                     KernelStatus* status) {
   constexpr int kN = Vec<T>::kN;
   Sums s{kLow, 0.f, 0.f, 0.f};
-  top = -CUDART_INF_F;
+  top = other = -CUDART_INF_F;
+  where = -1;
   float2 S2 = make_float2(0.f, 0.f), E2 = make_float2(0.f, 0.f);
   auto flush = [&]() {
     s.S += S2.x + S2.y;
     s.E += E2.x + E2.y;
     S2 = E2 = make_float2(0.f, 0.f);
   };
-  auto raise = [&](float m) {                                          // of the warp, where a lane's logits exceed it
+  auto raise = [&](float m, int at) {                                  // of the warp, where a lane's logits exceed it
+    const bool larger = top == top && !(m <= top);                     // NaN before all
+    other = larger ? top : max_nan(other, m);
+    where = larger ? at : where;
+    top = larger ? m : top;
     if (__any_sync(0xffffffffu, m > s.m)) {
       flush();
       for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -186,51 +247,46 @@ __device__ __forceinline__ Sums pass(const Part<T>& p, float& top) {
       E2 = fma2(y, e, E2);
     }
   };
-  const T* first = p.x + p.base;
-  const int turns = (p.pieces + kThreads - 1) / kThreads;
-  int j = threadIdx.x, done = 0;
-  // pieces 1 .. pieces - 2 are whole; a turn of kUnroll that all lie there is loaded at once
-  for (; done < turns;) {
-    const bool all = done > 0 && (done + kUnroll) * kThreads < p.pieces;
-    if (all) {
+  const int chunks = p.chunks();
+#pragma unroll 1
+  for (int c = 0; c < chunks; ++c, ++get) {
+    const int st = get % kStages, n = p.chunk_pieces(c) - static_cast<int>(threadIdx.x);
+    ok = ok && tc5::mbar_wait_warp(&sm.full[st], get / kStages & 1, &sm.abort_flag, status, STATUS_TIMEOUT_SMEM_FULL);
+    const uint4* at = ring + st * kChunk + threadIdx.x;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
       Vec<T> v[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) v[u] = load(first + static_cast<long>(j + u * kThreads) * kN);
-      float m = v[0].top();
+      for (int u = 0; u < kUnroll; ++u) *reinterpret_cast<uint4*>(&v[u].w) = at[(h * kUnroll + u) * kThreads];
+      if (h == kHalves - 1) tc5::arrive_warp(&sm.empty[st]);
+      if ((h + 1) * kUnroll * kThreads > n) {                          // what is behind the last piece is not this part's
 #pragma unroll
-      for (int u = 1; u < kUnroll; ++u) m = max_nan(m, v[u].top());
-      top = max_nan(top, m);
-      raise(m);
+        for (int u = 0; u < kUnroll; ++u)
+          if ((h * kUnroll + u) * kThreads >= n) v[u].clear();
+      }
+      raise(Vec<T>::top(v), c * kHalves + h);
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         float2 x[kN / 2];
         v[u].floats(x);
         add(x);
       }
-      j += kUnroll * kThreads;
-      done += kUnroll;
-    } else {
-      float2 x[kN / 2];
-      float m = -CUDART_INF_F;
-      if (j < p.pieces && p.whole(j)) {
-        const Vec<T> v = load(first + static_cast<long>(j) * kN);
-        m = v.top();
-        v.floats(x);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kN / 2; ++i) {
-          const int c = p.base + j * kN + 2 * i;
-          const float a = j < p.pieces ? p.at(c) : -CUDART_INF_F, b = j < p.pieces ? p.at(c + 1) : -CUDART_INF_F;
-          m = max_nan(m, max_nan(a, b));
-          x[i] = make_float2(max_nan(a, kLow), max_nan(b, kLow));
-        }
-      }
-      top = max_nan(top, m);
-      raise(m);
-      add(x);
-      j += kThreads;
-      done += 1;
     }
+  }
+  // the first and the last piece, where they are not whole
+  if (threadIdx.x < 64) {
+    float2 x[kN / 2];
+    float m = -CUDART_INF_F;
+    const int j = p.odd_piece(threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < kN / 2; ++i) {
+      const int c = p.base + j * kN + 2 * i;
+      const float a = j < 0 ? -CUDART_INF_F : p.at(c), b = j < 0 ? -CUDART_INF_F : p.at(c + 1);
+      m = max_nan(m, max_nan(a, b));
+      x[i] = make_float2(max_nan(a, kLow), max_nan(b, kLow));
+    }
+    raise(m, -1);
+    add(x);
   }
   flush();
   warp_reduce(s);
@@ -238,192 +294,315 @@ __device__ __forceinline__ Sums pass(const Part<T>& p, float& top) {
   return s;
 }
 
-// The part's k first in rank order, in sm.best (0 behind them).  top: the maximum of the thread's pieces.
+// The part's k first in rank order, in sm.best (0 behind them), by one warp.  top: the threads' maxima.
 template <class T>
-__device__ void select(Smem& sm, const Part<T>& p, float top, int k) {
-  constexpr int kN = Vec<T>::kN;
-  const int t = threadIdx.x, lane = t & 31, have = min(k, p.hi - p.lo);
-  const unsigned mine = ordered(top);
-  unsigned group = mine;
+__device__ __noinline__ void select(Smem& sm, const Part<T>& p, int b, int k) {
+  constexpr int kN = Vec<T>::kN, kEach = kThreads / 32;
+  constexpr unsigned kAll = 0xffffffffu;
+  static_assert(kEach == 4, "four maxima a lane");
+  const int lane = threadIdx.x & 31, have = min(k, p.hi - p.lo);
+  const uint4 four = *reinterpret_cast<const uint4*>(sm.top[b] + lane * 4), others = *reinterpret_cast<const uint4*>(sm.other[b] + lane * 4);
+  const unsigned mine[kEach] = {four.x, four.y, four.z, four.w}, second[kEach] = {others.x, others.y, others.z, others.w};
+  // the have-th largest of the pairs: the largest of all is taken out so many times (no logit's order is 0)
+  unsigned g0 = max(four.x, four.y), g1 = max(four.z, four.w), kth = 0;
+#pragma unroll 1
+  for (int n = 0; n < have; ++n) {
+    const unsigned m = max(g0, g1);
+    kth = __reduce_max_sync(kAll, m);
+    if (__ffs(__ballot_sync(kAll, m == kth)) - 1 == lane) {
+      if (g0 == kth) g0 = 0; else g1 = 0;
+    }
+  }
+  int reach = 0;
 #pragma unroll
-  for (int o = 1; o < kThreads / 64; o *= 2) group = max(group, __shfl_xor_sync(0xffffffffu, group, o));
-  if (t % (kThreads / 64) == 0) sm.group[t / (kThreads / 64)] = group;
-  if (t == 0) sm.count = sm.reach = sm.above = 0;
-  if (t < kTopMax) sm.best[t] = 0;
-  __syncthreads();
-  if (t < 64) {
-    const unsigned g = sm.group[t];
-    int before = 0;
-#pragma unroll 16
-    for (int i = 0; i < 64; ++i) before += sm.group[i] > g || (sm.group[i] == g && i < t);
-    if (before == have - 1) sm.kth = g;
+  for (int i = 0; i < kEach; ++i) reach += __popc(__ballot_sync(kAll, mine[i] >= kth));
+  // Logits that reach the bound.  Where far more threads' do than are asked for, logits are equal: then only those above it, and the first of the
+  // equal ones in order.
+  const bool ties = reach > 2 * have + 16;
+  const unsigned bound = ties ? kth : kth - 1;                         // candidates are larger than this
+  int n = 0, n_rest = 0, count = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const bool all = second[i] > bound, is = mine[i] > bound && !all;
+    const unsigned mask = __ballot_sync(kAll, is), mask_all = __ballot_sync(kAll, all), below = (1u << lane) - 1;
+    if (is) sm.list[n + __popc(mask & below)] = static_cast<short>(lane * 4 + i);
+    if (all) sm.rest[n_rest + __popc(mask_all & below)] = static_cast<short>(lane * 4 + i);
+    n += __popc(mask);
+    n_rest += __popc(mask_all);
   }
-  __syncthreads();
-  // Logits that reach the bound.  Where many threads' do, logits are equal: then only those above it, and the first of the equal ones in order.
-  const unsigned kth = sm.kth;
-  if (mine >= kth) atomicAdd(&sm.reach, 1);
-  __syncthreads();
-  const bool ties = sm.reach > 3 * kTopMax;
-  const unsigned bound = ties ? kth : kth - 1;                         // candidates are larger than this (no logit's order is 0)
-  if (mine > bound) sm.list[atomicAdd(&sm.above, 1)] = static_cast<short>(t);
-  __syncthreads();
-  const int turns = (p.pieces + kThreads - 1) / kThreads, again = sm.above * turns;
-  for (int i = t; i < again; i += kThreads) {
-    const int j = sm.list[i / turns] + i % turns * kThreads;
-    if (j >= p.pieces) continue;
-    for (int c = 0; c < kN; ++c) {
-      const int col = p.base + j * kN + c;
-      if (col < p.lo || col >= p.hi) continue;
-      const float x = value(p.x, col);
-      if (ordered(x) > bound) {
-        const int at = atomicAdd(&sm.count, 1);
-        if (at < kBuffer) sm.buffer[at] = rank_of(x, col);
+  sm.best[lane] = 0;
+  __syncwarp();
+  auto candidate = [&](bool is, float x, int col) {                    // of all lanes at once
+    is = is && col >= p.lo && col < p.hi;
+    const unsigned mask = __ballot_sync(kAll, is);
+    const int at = count + __popc(mask & ((1u << lane) - 1));
+    if (is && at < kBuffer) sm.buffer[at] = rank_of(x, col);
+    count += __popc(mask);
+  };
+  constexpr int kAtOnce = 4;                                           // loads of a lane
+  auto look = [&](const Vec<T> (&v)[kAtOnce], const int (&j)[kAtOnce]) {                 // j: pieces, -1: none
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      float2 x[kN / 2];
+      v[i].exact(x);
+      unsigned hits = 0;
+#pragma unroll
+      for (int c = 0; c < kN / 2; ++c) hits |= (ordered(x[c].x) > bound ? 1u << 2 * c : 0u) | (ordered(x[c].y) > bound ? 2u << 2 * c : 0u);
+      if (j[i] < 0) hits = 0;
+      while (__any_sync(kAll, hits)) {                                 // one of each lane's
+        const int c = hits ? __ffs(hits) - 1 : 0;
+        float value = x[0].x;
+#pragma unroll
+        for (int y = 1; y < kN; ++y) value = c == y ? (y & 1 ? x[y / 2].y : x[y / 2].x) : value;
+        candidate(hits != 0, value, p.base + j[i] * kN + c);
+        hits &= hits - 1;
       }
     }
-  }
-  __syncthreads();
-  int count = sm.count;
-  if (count <= kBuffer) {
-    if (ties && count < have) {
-      const int missing = have - count;
-      int found = 0;
-      for (int c0 = p.lo; c0 < p.hi && found < missing; c0 += kThreads) {
-        const bool is = c0 + t < p.hi && ordered(value(p.x, c0 + t)) == kth;
-        const unsigned mask = __ballot_sync(0xffffffffu, is);
-        if (lane == 0) sm.red[t >> 5] = __popc(mask);
-        __syncthreads();
-        int before = found;
-        for (int w = 0; w < kWarps; ++w) {
-          if (w < (t >> 5)) before += static_cast<int>(sm.red[w]);
-          found += static_cast<int>(sm.red[w]);
-        }
-        const int at = before + __popc(mask & ((1u << lane) - 1));
-        if (is && at < missing) sm.buffer[count + at] = rank_of(value(p.x, c0 + t), c0 + t);
-        __syncthreads();
-      }
-      count += min(found, missing);
+  };
+  // the four pieces of a thread's largest logit: a lane takes those of one thread
+#pragma unroll 1
+  for (int e = 0; e < n; e += 32) {
+    Vec<T> v[kAtOnce];
+    int j[kAtOnce];
+    const int who = e + lane < n ? sm.list[e + lane] : 0, half = e + lane < n ? sm.where[b][who] : -1;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      j[i] = p.w0 + who + (half * kUnroll + i) * kThreads;
+      if (half < 0 || j[i] >= p.w1) j[i] = -1;
+      v[i].clear();
+      if (j[i] >= 0) v[i] = load(p.x + p.base + j[i] * kN);
     }
-    for (int i = t; i < count; i += kThreads) {
+    look(v, j);
+  }
+  // all pieces of the others
+  const int turns = (p.w1 - p.w0 + kThreads - 1) / kThreads;
+#pragma unroll 1
+  for (int e = 0; e < n_rest; ++e)
+#pragma unroll 1
+    for (int turn = 0; turn < turns; turn += 32 * kAtOnce) {
+      Vec<T> v[kAtOnce];
+      int j[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        j[i] = p.w0 + sm.rest[e] + (turn + i * 32 + lane) * kThreads;
+        if (j[i] >= p.w1) j[i] = -1;
+        v[i].clear();
+        if (j[i] >= 0) v[i] = load(p.x + p.base + j[i] * kN);
+      }
+      look(v, j);
+    }
+  {                                                                    // the pieces that are not whole: a column per lane
+    const int j = p.odd_piece(lane < kN ? 0 : 32), col = p.base + j * kN + lane % kN;
+    const float x = j >= 0 && lane < 2 * kN ? p.at(col) : -CUDART_INF_F;
+    candidate(j >= 0 && lane < 2 * kN && ordered(x) > bound, x, col);
+  }
+  if (count <= kBuffer - kTopMax) {
+    if (ties)
+      for (int c0 = p.lo; c0 < p.hi && count < have; c0 += 32) {
+        const float x = p.at(c0 + lane);
+        candidate(ordered(x) == kth, x, c0 + lane);
+      }
+    __syncwarp();
+#pragma unroll 1
+    for (int i = lane; i < count; i += 32) {
       const u64 r = sm.buffer[i];
       int before = 0;
+#pragma unroll 8
       for (int o = 0; o < count; ++o) before += sm.buffer[o] > r;
       if (before < have) sm.best[before] = r;
     }
-    __syncthreads();
+    __syncwarp();
     return;
   }
-  // more candidates than are kept (the largest logits all in one thread's pieces): one after another
+  // more candidates than are kept (the largest logits all in few threads' pieces): one after another
   u64 last = ~0ull;
-  for (int n = 0; n < have; ++n) {
+  for (int m = 0; m < have; ++m) {
     u64 r = 0;
-    for (int c = p.lo + t; c < p.hi; c += kThreads) {
+    for (int c = p.lo + lane; c < p.hi; c += 32) {
       const u64 a = rank_of(value(p.x, c), c);
       if (a < last && a > r) r = a;
     }
     for (int o = 16; o; o >>= 1) {
-      const u64 a = __shfl_xor_sync(0xffffffffu, r, o);
+      const u64 a = __shfl_xor_sync(kAll, r, o);
       r = a > r ? a : r;
     }
-    __syncthreads();
-    if (lane == 0) sm.red[t >> 5] = r;
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w) r = sm.red[w] > r ? sm.red[w] : r;
     last = r;
-    if (t == 0) sm.best[n] = r;
+    if (lane == 0) sm.best[m] = r;
   }
-  __syncthreads();
+  __syncwarp();
 }
 
-// One row per cluster, its columns in even parts.
+// A row's end, by one warp: a are its sums, sm.best of the cluster's CTAs its candidates.
 template <class T>
-__global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(const T* __restrict__ logits, long ld, const long long* __restrict__ tokens,
-                                                                   float* __restrict__ logprob, float* __restrict__ entropy, float2* __restrict__ stats,
-                                                                   float* __restrict__ top_out, long long* __restrict__ index, int V, int k,
-                                                                   long long ignore, int parts, KernelStatus* status) {
+__device__ __noinline__ void finish(Smem& sm, Sums a, const T* x, long row, long long tok, float chosen, float* logprob, float* entropy, float2* stats, float* top_out,
+                                    long long* index, int V, int k, long long ignore, int parts, KernelStatus* status) {
+  const int lane = threadIdx.x & 31;
+  float m = a.m, logS = logf(a.S) - fmaf(m, kLog2e, -a.R) * kLn2, H = logf(a.S);
+  bool empty = false;
+  if (m <= 0.1f * kLow) {                                              // near kLow the pass has not told logits apart
+    m = -CUDART_INF_F;
+    for (int c = lane; c < V; c += 32) m = max_nan(m, value(x, c));
+    for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    empty = m == -CUDART_INF_F;
+    Sums b{0.f, 0.f, 0.f, 0.f};
+    for (int c = lane; c < V && !empty; c += 32) {
+      const float y = (value(x, c) - m) * kLog2e, e = ex2(y);
+      b.S += e;
+      b.E += e > 0.f ? y * e : e;
+    }
+    warp_reduce(b);
+    a = b;
+    H = logS = empty ? 0.f : logf(a.S);
+  }
+  H = empty ? 0.f : H - a.E * kLn2 / a.S;
+  if (lane == 0) {
+    NSA_CHECK_INDEX(tok == ignore || (tok >= 0 && tok < V), status, tok);
+    logprob[row] = tok == ignore || tok < 0 || tok >= V ? 0.f : empty ? m : chosen - m - logS;
+    entropy[row] = H;
+    stats[row] = make_float2(m, logS);                                 // apart: their sum would round a probability by |m| 2^-24
+  }
+  if (k == 0) return;
+  auto put = [&](int place, u64 r) {
+    index[row * k + place] = index_of(r);
+    top_out[row * k + place] = empty ? m : logit_of(r) - m - logS;
+  };
+  if (parts == 1) {
+    if (lane < k) put(lane, sm.best[lane]);
+    return;
+  }
+  // each part's best are in order: a candidate's place is its own, and the number of larger ones in each other part
+  const int n = parts * k;
+  for (int i = lane; i < n; i += 32) sm.buffer[i] = *cg::this_cluster().map_shared_rank(&sm.best[i % k], i / k);
+  __syncwarp();
+  for (int i = lane; i < n; i += 32) {
+    const u64 r = sm.buffer[i];
+    int before = i % k;
+    for (int c = 0; c < parts; ++c) {
+      if (c == i / k) continue;
+      int lo = 0, hi = k;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sm.buffer[c * k + mid] > r) lo = mid + 1; else hi = mid;
+      }
+      before += lo;
+    }
+    if (r != 0 && before < k) put(before, r);
+  }
+  __syncwarp();
+}
+
+// A cluster takes a row at a time, its CTAs even parts of the columns.
+template <class T>
+__global__ void __launch_bounds__(kThreads + 64, kCtas) logprobs_fwd_kernel(const T* __restrict__ logits, long ld, const long long* __restrict__ tokens,
+                                                                            float* __restrict__ logprob, float* __restrict__ entropy,
+                                                                            float2* __restrict__ stats, float* __restrict__ top_out,
+                                                                            long long* __restrict__ index, long rows, int V, int k, long long ignore,
+                                                                            int parts, KernelStatus* status) {
+  extern __shared__ __align__(128) uint4 ring[];
   __shared__ Smem sm;
-  const int t = threadIdx.x, part = blockIdx.x % parts;
-  const long row = blockIdx.x / parts;
-  const T* x = logits + row * ld;
-  const int each = (V + parts - 1) / parts;
-  const Part<T> p(x, min(part * each, V), min((part + 1) * each, V));
-  float top;
-  const Sums s = pass(p, top);
-  if ((t & 31) == 0) sm.sums[t >> 5] = s;
-  if (k > 0) select(sm, p, top, k);
-  __syncthreads();
+  const int t = threadIdx.x, lane = t & 31, warp = tc5::warp_index(), part = blockIdx.x % parts;
+  const long first = blockIdx.x / parts, step = gridDim.x / parts;
+  const int each = (V + parts - 1) / parts, lo = min(part * each, V), hi = min((part + 1) * each, V);
   if (t == 0) {
-    Sums a = sm.sums[0];
-    for (int w = 1; w < kWarps; ++w) a.add(sm.sums[w]);
-    sm.all = a;
-  }
-  if (parts > 1) {
-    cg::this_cluster().sync();
-  } else {
-    __syncthreads();
-  }
-  if (part == 0) {
-    Sums a = sm.all;
-    for (int c = 1; c < parts; ++c) a.add(*cg::this_cluster().map_shared_rank(&sm.all, c));
-    // near kLow the pass has not told logits apart
-    float m = a.m, logS = logf(a.S) - fmaf(m, kLog2e, -a.R) * kLn2, H = logf(a.S);
-    bool empty = false;
-    if (m <= 0.1f * kLow) {
-      m = -CUDART_INF_F;
-      for (int c = t; c < V; c += kThreads) m = max_nan(m, value(x, c));
-      sm.top[t] = m;
-      __syncthreads();
-      for (int i = 0; i < kThreads; ++i) m = max_nan(m, sm.top[i]);
-      empty = m == -CUDART_INF_F;
-      float S = 0.f, E = 0.f;
-      for (int c = t; c < V && !empty; c += kThreads) {
-        const float y = (value(x, c) - m) * kLog2e, e = ex2(y);
-        S += e;
-        E += e > 0.f ? y * e : e;
-      }
-      Sums b{0.f, 0.f, S, E};
-      warp_reduce(b);
-      __syncthreads();
-      if ((t & 31) == 0) sm.sums[t >> 5] = b;
-      __syncthreads();
-      b = Sums{0.f, 0.f, 0.f, 0.f};
-      for (int w = 0; w < kWarps; ++w) {
-        b.S += sm.sums[w].S;
-        b.E += sm.sums[w].E;
-      }
-      a = b;
-      H = logS = empty ? 0.f : logf(a.S);
+    sm.abort_flag = 0;
+    for (int i = 0; i < kStages; ++i) {
+      tc5::mbar_init(&sm.full[i], 1);
+      tc5::mbar_init(&sm.empty[i], kWarps);
     }
-    H = empty ? 0.f : H - a.E * kLn2 / a.S;
-    if (t == 0) {
-      const long long tok = tokens[row];
-      NSA_CHECK_INDEX(tok == ignore || (tok >= 0 && tok < V), status, tok);
-      logprob[row] = tok == ignore || tok < 0 || tok >= V ? 0.f : empty ? m : value(x, tok) - m - logS;
-      entropy[row] = H;
-      stats[row] = make_float2(m, logS);                               // apart: their sum would round a probability by |m| 2^-24
+    for (int i = 0; i < 2; ++i) {
+      tc5::mbar_init(&sm.ready[i], kWarps);
+      tc5::mbar_init(&sm.taken[i], 1);
     }
-    // each part's best are in order: a candidate's place is the number of larger ones
-    const int n = parts * k;
-    for (int i = t; i < n; i += kThreads) sm.buffer[i] = *cg::this_cluster().map_shared_rank(&sm.best[i % k], i / k);
-    __syncthreads();
-    for (int i = t; i < n; i += kThreads) {
-      const u64 r = sm.buffer[i];
-      if (r == 0) continue;
-      int before = 0;
-      for (int o = 0; o < n; ++o) before += sm.buffer[o] > r;
-      if (before < k) {
-        const int c = index_of(r);
-        index[row * k + before] = c;
-        top_out[row * k + before] = empty ? m : value(x, c) - m - logS;
+    tc5::fence_barrier_init();
+  }
+  __syncthreads();
+  bool ok = true;
+  uint32_t n = 0;                                                      // rows that this CTA has had
+  if (warp < kWarps) {
+    uint32_t get = 0;
+#pragma unroll 1
+    for (long row = first; row < rows; row += step, ++n) {
+      const Part<T> p(logits + row * ld, lo, hi);
+      float top, other;
+      int where;
+      const Sums s = pass(p, sm, ring, get, ok, top, other, where, status);
+      const int b = n & 1;
+      if (n >= 2) ok = ok && tc5::mbar_wait_warp(&sm.taken[b], (n / 2 - 1) & 1, &sm.abort_flag, status, STATUS_TIMEOUT_SMEM_EMPTY);
+      sm.top[b][t] = ordered(top);
+      sm.other[b][t] = ordered(other);
+      sm.where[b][t] = static_cast<short>(where);
+      if (lane == 0) sm.sums[b][warp] = s;
+      tc5::arrive_warp(&sm.ready[b]);
+      if (parts > 1) {
+        cg::this_cluster().sync();
+        cg::this_cluster().sync();
       }
     }
+  } else if (warp == kWarps) {                                         // the copies
+    uint32_t put = 0;
+#pragma unroll 1
+    for (long row = first; row < rows; row += step) {
+      if (lane == 0) {
+        const Part<T> p(logits + row * ld, lo, hi);
+        const int chunks = p.chunks();
+        for (int c = 0; c < chunks && ok; ++c, ++put) {
+          const int st = put % kStages, bytes = p.chunk_pieces(c) * 16;
+          if (put >= kStages) ok = tc5::mbar_wait(&sm.empty[st], (put / kStages - 1) & 1, &sm.abort_flag, status, STATUS_TIMEOUT_SMEM_EMPTY);
+          if (!ok) break;
+          tc5::mbar_expect_tx(&sm.full[st], bytes);
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc5::smem_u32(ring + st * kChunk)),
+                       "l"(p.chunk(c)), "r"(bytes), "r"(tc5::smem_u32(&sm.full[st]))
+                       : "memory");
+        }
+      }
+      __syncwarp();
+      if (parts > 1) {
+        cg::this_cluster().sync();
+        cg::this_cluster().sync();
+      }
+    }
+    if (lane == 0 && sm.abort_flag)
+      for (int i = 0; i < kStages; ++i) tc5::mbar_drain(&sm.full[i]);
+  } else {                                                             // the rows' ends
+    // the given token of the row after the next and its logit of the next one are on their way meanwhile
+    auto token = [&](long row) { return row < rows ? tokens[row] : -1ll; };
+    auto logit = [&](long row, long long tok) { return tok >= 0 && tok < V ? value(logits + row * ld, tok) : 0.f; };
+    long long tok = token(first), tok1 = token(first + step);
+    float chosen = logit(first, tok);
+#pragma unroll 1
+    for (long row = first; row < rows; row += step, ++n) {
+      const T* x = logits + row * ld;
+      const int b = n & 1;
+      const long long tok2 = token(row + 2 * step);
+      const float chosen1 = logit(row + step, tok1);
+      // most of the time there is nothing to do: polling would take the others' issue slots
+      for (int i = 0; i < 20000 && !__all_sync(0xffffffffu, tc5::mbar_try_wait(&sm.ready[b], n / 2 & 1)); ++i) __nanosleep(100);
+      ok = ok && tc5::mbar_wait_warp(&sm.ready[b], n / 2 & 1, &sm.abort_flag, status, STATUS_TIMEOUT_SMEM_FULL);
+      if (ok) {
+        Sums a = sm.sums[b][0];
+        for (int w = 1; w < kWarps; ++w) a.add(sm.sums[b][w]);
+        sm.all = a;
+        if (k > 0) select(sm, Part<T>(x, lo, hi), b, k);
+      }
+      if (parts > 1) cg::this_cluster().sync();
+      if (part == 0 && ok) {
+        Sums a = sm.all;
+        for (int c = 1; c < parts; ++c) a.add(*cg::this_cluster().map_shared_rank(&sm.all, c));
+        finish(sm, a, x, row, tok, chosen, logprob, entropy, stats, top_out, index, V, k, ignore, parts, status);
+      }
+      if (parts > 1) cg::this_cluster().sync();                        // the others' memory is read until here
+      tc5::arrive_warp(&sm.taken[b]);
+      tok = tok1;
+      tok1 = tok2;
+      chosen = chosen1;
+    }
   }
-  if (parts > 1) cg::this_cluster().sync();                            // the others' memory is read until here
 }
 
 // dx_j = -p_j (G + g_H (log p_j + H)), G the sum of the row's other gradients; theirs are added at their tokens.  One CTA per kBwdPieces pieces of a row.
-constexpr int kBwdTurns = 4, kBwdPieces = kThreads * kBwdTurns;
+constexpr int kBwdThreads = 256, kBwdTurns = 4, kBwdPieces = kBwdThreads * kBwdTurns;
 template <class T>
-__global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const T* __restrict__ logits, long ld, const long long* __restrict__ tokens,
+__global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const T* __restrict__ logits, long ld, const long long* __restrict__ tokens,
                                                                 const float2* __restrict__ stats, const float* __restrict__ entropy,
                                                                 const long long* __restrict__ index, const float* __restrict__ dlogprob,
                                                                 const float* __restrict__ dentropy, const float* __restrict__ dtop,
@@ -434,6 +613,18 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const T* __restr
   const int chunk = static_cast<int>(blockIdx.x - row * chunks);
   const T* x = logits + row * ld;
   T* dx = dx_all + row * V;
+  // pieces where dx is 16-byte aligned; x is as well, or its elements are loaded one by one
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(dx) % 16 / sizeof(T)), pieces = (V + off + kN - 1) / kN;
+  const bool same = (reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) % 16 == 0;
+  const int j0 = chunk * kBwdPieces;
+  Vec<T> v[kBwdTurns];
+  bool whole[kBwdTurns];
+#pragma unroll
+  for (int u = 0; u < kBwdTurns; ++u) {
+    const int j = j0 + u * kBwdThreads + t, c = j * kN - off;
+    whole[u] = same && c >= 0 && c + kN <= V;
+    if (whole[u]) v[u] = load(x + c);
+  }
   const float m = stats[row].x, logS = stats[row].y, H = entropy[row], gH = dentropy ? dentropy[row] : 0.f;
   const long long tok = tokens[row];
   const bool counts = !(tok == ignore || tok < 0 || tok >= V), empty = m == -CUDART_INF_F;
@@ -447,29 +638,16 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const T* __restr
     const float y = max_nan(fmaf(v - m, kLog2e, -log2S), -1000.f);
     return ex2_small(y) * fmaf(c2, y, c1);
   };
-  // pieces where dx is 16-byte aligned; x is as well, or its elements are loaded one by one
-  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(dx) % 16 / sizeof(T)), pieces = (V + off + kN - 1) / kN;
-  const bool same = (reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) % 16 == 0;
-  const int j0 = chunk * kBwdPieces;
-  Vec<T> v[kBwdTurns];
-  bool whole[kBwdTurns];
 #pragma unroll
   for (int u = 0; u < kBwdTurns; ++u) {
-    const int j = j0 + u * kThreads + t, c = j * kN - off;
-    whole[u] = same && c >= 0 && c + kN <= V;
-    if (whole[u]) v[u] = load(x + c);
-  }
-#pragma unroll
-  for (int u = 0; u < kBwdTurns; ++u) {
-    const int j = j0 + u * kThreads + t, c = j * kN - off;
+    const int j = j0 + u * kBwdThreads + t, c = j * kN - off;
     if (j >= pieces) break;
     if (whole[u]) {
-      const T* in = reinterpret_cast<const T*>(&v[u].w);
-      Vec<T> out;
-      T* o = reinterpret_cast<T*>(&out.w);
+      float2 a[kN / 2];
+      v[u].exact(a);
 #pragma unroll
-      for (int i = 0; i < kN; ++i) store(o, i, empty ? 0.f : grad(value(in, i)));
-      __stcs(reinterpret_cast<uint4*>(dx + c), *reinterpret_cast<const uint4*>(&out.w));
+      for (int i = 0; i < kN / 2; ++i) a[i] = empty ? make_float2(0.f, 0.f) : make_float2(grad(a[i].x), grad(a[i].y));
+      __stcs(reinterpret_cast<uint4*>(dx + c), Vec<T>::pack(a));
     } else {
       for (int i = 0; i < kN; ++i)
         if (c + i >= 0 && c + i < V) store(dx, c + i, empty ? 0.f : grad(value(x, c + i)));
@@ -479,7 +657,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const T* __restr
   __syncthreads();
   // the chosen token (t = k) and the likeliest ones, each column once
   const int n = dtop ? k : 0;
-  for (int i = t; i <= n; i += kThreads) {
+  for (int i = t; i <= n; i += kBwdThreads) {
     if (i == n && !counts) continue;
     const long long c = i == n ? tok : index[row * k + i];
     const long piece = (c + off) / kN;
@@ -501,10 +679,12 @@ cudaError_t forward(const void* logits, long ld, const long long* tokens, float*
   // CTAs of a row: with fewer rows than SMs up to 8, of 4096 columns at least
   const int sms = nsa::sm_count();
   int parts = 1;
-  while (parts < 8 && rows * parts * 2 <= 2l * sms && V / (2 * parts) >= 4096) parts *= 2;
+  while (parts < 8 && rows * parts * 2 <= static_cast<long>(kCtas) * sms && V / (2 * parts) >= 4096) parts *= 2;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = static_cast<unsigned>(rows * parts);
-  cfg.blockDim = kThreads;
+  const long most = static_cast<long>(kCtas) * sms / parts;
+  cfg.gridDim = static_cast<unsigned>((rows < most ? rows : most) * parts);
+  cfg.dynamicSmemBytes = kStages * kChunk * 16;
+  cfg.blockDim = kThreads + 64;
   cfg.stream = st;
   cudaLaunchAttribute cluster{};
   cluster.id = cudaLaunchAttributeClusterDimension;
@@ -512,15 +692,23 @@ cudaError_t forward(const void* logits, long ld, const long long* tokens, float*
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   cfg.attrs = &cluster;
   cfg.numAttrs = 1;
+  static std::atomic<unsigned long long> ready{0};                     // devices on which the kernel may have this much shared memory
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    const cudaError_t e = cudaFuncSetAttribute(logprobs_fwd_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStages * kChunk * 16);
+    if (e != cudaSuccess) return e;
+    if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   return cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T>, static_cast<const T*>(logits), ld, tokens, logprob, entropy, reinterpret_cast<float2*>(stats), top,
-                            index, V, k, ignore, parts, nsa::status_ptr());
+                            index, rows, V, k, ignore, parts, nsa::status_ptr());
 }
 }  // namespace
 
 extern "C" int nsa_logprobs_fwd(const void* logits, long ld, int fp32, const long long* tokens, float* logprob, float* entropy, float* stats, float* top,
                                 long long* index, long rows, int V, int k, long long ignore, cudaStream_t st) {
   if (rows <= 0) return 0;
-  if (V <= 0 || V > 0x7fff0000 || k < 0 || k > V || k > kTopMax || rows > 0x7fffffff) return nsa::fail(NSA_ERR_SHAPE, "logprobs: unsupported shape");
+  if (V <= 0 || V > kWidest || k < 0 || k > V || k > kTopMax || rows > 0x7fffffff) return nsa::fail(NSA_ERR_SHAPE, "logprobs: unsupported shape");
   const cudaError_t e = fp32 ? forward<float>(logits, ld, tokens, logprob, entropy, stats, top, index, rows, V, k, ignore, st)
                              : forward<bf16>(logits, ld, tokens, logprob, entropy, stats, top, index, rows, V, k, ignore, st);
   if (e != cudaSuccess) return nsa::fail_cuda(e, "nsa_logprobs_fwd launch");
@@ -537,10 +725,10 @@ extern "C" int nsa_logprobs_bwd(const void* logits, long ld, int fp32, const lon
   if (rows * chunks > 0x7fffffff) return nsa::fail(NSA_ERR_SHAPE, "logprobs: unsupported shape");
   const unsigned grid = static_cast<unsigned>(rows * chunks);
   if (fp32)
-    logprobs_bwd_kernel<<<grid, kThreads, 0, st>>>(static_cast<const float*>(logits), ld, tokens, reinterpret_cast<const float2*>(stats), entropy, index,
+    logprobs_bwd_kernel<<<grid, kBwdThreads, 0, st>>>(static_cast<const float*>(logits), ld, tokens, reinterpret_cast<const float2*>(stats), entropy, index,
                                                    dlogprob, dentropy, dtop, static_cast<float*>(dx), V, k, ignore, chunks);
   else
-    logprobs_bwd_kernel<<<grid, kThreads, 0, st>>>(static_cast<const bf16*>(logits), ld, tokens, reinterpret_cast<const float2*>(stats), entropy, index,
+    logprobs_bwd_kernel<<<grid, kBwdThreads, 0, st>>>(static_cast<const bf16*>(logits), ld, tokens, reinterpret_cast<const float2*>(stats), entropy, index,
                                                    dlogprob, dentropy, dtop, static_cast<bf16*>(dx), V, k, ignore, chunks);
   nsa::count_launch();
   const cudaError_t e = cudaGetLastError();
