@@ -140,10 +140,8 @@ __device__ __forceinline__ unsigned ordered(float x) {
   return bits >= 0 ? static_cast<unsigned>(bits) | 0x80000000u : ~static_cast<unsigned>(bits);
 }
 __device__ __forceinline__ u64 rank_of(float x, int i) { return static_cast<u64>(ordered(x)) << 32 | (0xffffffffu - static_cast<unsigned>(i)); }
-__device__ __forceinline__ float logit_of(u64 r) {
-  const unsigned o = static_cast<unsigned>(r >> 32);
-  return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o);
-}
+__device__ __forceinline__ float number_of(unsigned o) { return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o); }
+__device__ __forceinline__ float logit_of(u64 r) { return number_of(static_cast<unsigned>(r >> 32)); }
 __device__ __forceinline__ int index_of(u64 r) { return static_cast<int>(0xffffffffu - static_cast<unsigned>(r)); }
 
 // Sums over some logits, of which m is the largest; none yet (or none above kLow) where m is kLow
@@ -320,6 +318,9 @@ __device__ __noinline__ void select(Smem& sm, const Part<T>& p, int b, int k) {
   // equal ones in order.
   const bool ties = reach > 2 * have + 16;
   const unsigned bound = ties ? kth : kth - 1;                         // candidates are larger than this
+  // the same as a test of numbers, !(x <= under): NaN is larger than any (bound < NaN's order: no number lies between infinity's and it), zeros are equal
+  const bool none = bound == 0xffffffffu;
+  const float under = bound >= 0xff800000u ? CUDART_INF_F : bound == 0x7fffffffu ? -1.401298e-45f : number_of(bound);
   int n = 0, n_rest = 0, count = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
@@ -341,22 +342,28 @@ __device__ __noinline__ void select(Smem& sm, const Part<T>& p, int b, int k) {
   };
   constexpr int kAtOnce = 4;                                           // loads of a lane
   auto look = [&](const Vec<T> (&v)[kAtOnce], const int (&j)[kAtOnce]) {                 // j: pieces, -1: none
+    unsigned hits = 0;
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       float2 x[kN / 2];
       v[i].exact(x);
-      unsigned hits = 0;
 #pragma unroll
-      for (int c = 0; c < kN / 2; ++c) hits |= (ordered(x[c].x) > bound ? 1u << 2 * c : 0u) | (ordered(x[c].y) > bound ? 2u << 2 * c : 0u);
-      if (j[i] < 0) hits = 0;
-      while (__any_sync(kAll, hits)) {                                 // one of each lane's
-        const int c = hits ? __ffs(hits) - 1 : 0;
-        float value = x[0].x;
-#pragma unroll
-        for (int y = 1; y < kN; ++y) value = c == y ? (y & 1 ? x[y / 2].y : x[y / 2].x) : value;
-        candidate(hits != 0, value, p.base + j[i] * kN + c);
-        hits &= hits - 1;
+      for (int c = 0; c < kN / 2; ++c) {
+        if (!(x[c].x <= under)) hits |= 1u << (i * kN + 2 * c);
+        if (!(x[c].y <= under)) hits |= 2u << (i * kN + 2 * c);
       }
+      if (j[i] < 0) hits &= ~(((1u << kN) - 1) << (i * kN));
+    }
+    if (none) hits = 0;
+#pragma unroll 1
+    while (__any_sync(kAll, hits)) {                                   // one of each lane's; the number is read again, from L1
+      const int at = hits ? __ffs(hits) - 1 : 0;
+      int piece = j[0];
+#pragma unroll
+      for (int i = 1; i < kAtOnce; ++i) piece = at / kN == i ? j[i] : piece;
+      const int col = p.base + piece * kN + at % kN;
+      candidate(hits != 0, hits ? value(p.x, col) : 0.f, col);
+      hits &= hits - 1;
     }
   };
   // the four pieces of a thread's largest logit: a lane takes those of one thread
@@ -470,24 +477,32 @@ __device__ __noinline__ void finish(Smem& sm, Sums a, const T* x, long row, long
     if (lane < k) put(lane, sm.best[lane]);
     return;
   }
-  // each part's best are in order: a candidate's place is its own, and the number of larger ones in each other part
+  // each part's best are in order: the best of their heads k times
   const int n = parts * k;
-  for (int i = lane; i < n; i += 32) sm.buffer[i] = *cg::this_cluster().map_shared_rank(&sm.best[i % k], i / k);
-  __syncwarp();
-  for (int i = lane; i < n; i += 32) {
-    const u64 r = sm.buffer[i];
-    int before = i % k;
-    for (int c = 0; c < parts; ++c) {
-      if (c == i / k) continue;
-      int lo = 0, hi = k;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (sm.buffer[c * k + mid] > r) lo = mid + 1; else hi = mid;
-      }
-      before += lo;
-    }
-    if (r != 0 && before < k) put(before, r);
+#pragma unroll
+  for (int i = 0; i < 8 * kTopMax / 32; ++i) {
+    const int at = i * 32 + lane;
+    if (at < n) sm.buffer[at] = *cg::this_cluster().map_shared_rank(&sm.best[at % k], at / k);
   }
+  __syncwarp();
+  int next = 1;
+  u64 head = lane < parts ? sm.buffer[lane * k] : 0, mine = 0;
+#pragma unroll 1
+  for (int place = 0; place < k; ++place) {
+    u64 r = head;
+#pragma unroll
+    for (int o = 4; o; o >>= 1) {
+      const u64 a = __shfl_xor_sync(0xffffffffu, r, o);
+      r = a > r ? a : r;
+    }
+    r = __shfl_sync(0xffffffffu, r, 0);
+    if (lane == place) mine = r;
+    if (head == r && lane < parts) {
+      head = next < k ? sm.buffer[lane * k + next] : 0;
+      ++next;
+    }
+  }
+  if (lane < k) put(lane, mine);
   __syncwarp();
 }
 
@@ -587,7 +602,11 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) logprobs_fwd_kernel(cons
       if (parts > 1) cg::this_cluster().sync();
       if (part == 0 && ok) {
         Sums a = sm.all;
-        for (int c = 1; c < parts; ++c) a.add(*cg::this_cluster().map_shared_rank(&sm.all, c));
+        if (parts > 1) {                                               // lane c fetches part c's
+          const Sums o = *cg::this_cluster().map_shared_rank(&sm.all, lane < parts ? lane : 0);
+          for (int c = 1; c < parts; ++c)
+            a.add(Sums{__shfl_sync(0xffffffffu, o.m, c), __shfl_sync(0xffffffffu, o.R, c), __shfl_sync(0xffffffffu, o.S, c), __shfl_sync(0xffffffffu, o.E, c)});
+        }
         finish(sm, a, x, row, tok, chosen, logprob, entropy, stats, top_out, index, V, k, ignore, parts, status);
       }
       if (parts > 1) cg::this_cluster().sync();                        // the others' memory is read until here
