@@ -8,34 +8,37 @@ namespace {
 typedef __nv_bfloat16 bf16;
 
 // ------------------------------------------------------------------------------------- pages and slots of a step
+// A few thousand numbers at most: what counts is the chain of dependent loads (lengths and counts together, then a page number) and barriers, so each
+// CTA scans all requests by itself and no CTA waits for another.  XX
 constexpr int kPlanThreads = 1024;
 
-// Exclusive prefix of two values per thread over the CTA, and their totals
-__device__ __forceinline__ void scan2(long long& a, long long& b, long long& ta, long long& tb, long long (*warps)[2]) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  long long x = a, y = b;
+// Exclusive prefix of a value per thread over the CTA, and the total
+template <class T>
+__device__ __forceinline__ T scan(T mine, T& total, T* warps) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, n = blockDim.x >> 5;
+  T x = mine;
+#pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, x, d), v = __shfl_up_sync(0xffffffffu, y, d);
-    if (lane >= d) { x += u; y += v; }
+    const T u = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += u;
   }
-  if (lane == 31) { warps[w][0] = x; warps[w][1] = y; }
+  if (lane == 31) warps[w] = x;
   __syncthreads();
-  long long bx = 0, by = 0;
-  ta = tb = 0;
-  for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) {
-    if (i < w) { bx += warps[i][0]; by += warps[i][1]; }
-    ta += warps[i][0];
-    tb += warps[i][1];
+  T y = lane < n ? warps[lane] : 0;                                    // each warp scans the warps' sums
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const T u = __shfl_up_sync(0xffffffffu, y, d);
+    if (lane >= d) y += u;
   }
-  __syncthreads();
-  a = bx + x - a;
-  b = by + y - b;
+  total = __shfl_sync(0xffffffffu, y, 31);
+  const T before = __shfl_sync(0xffffffffu, y, w ? w - 1 : 0);
+  return x - mine + (w ? before : 0);
 }
 
 __device__ __forceinline__ int pages_for(long long tokens, int shift) { return static_cast<int>((tokens + (1 << shift) - 1) >> shift); }
 
-// Every CTA scans all requests (start[b], and first[b]: new pages of the requests before b, both in shared memory) and writes its share of the
-// table's new entries and of the slots.
+// Every CTA scans all requests (first token, first new page and length of each in shared memory) and writes its share of the table's new entries and of
+// the slots.
 __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const int* __restrict__ lengths, const int* __restrict__ add, int* __restrict__ table,
                                                                   const int* __restrict__ free_pages, const int* __restrict__ free_count, int F,
                                                                   int* __restrict__ query_start, int* __restrict__ total,
@@ -43,23 +46,24 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const int* __r
                                                                   int* __restrict__ free_left, int* __restrict__ shortfall, int B, int W, int N,
                                                                   int shift) {
   extern __shared__ int plan_smem[];
-  __shared__ long long warps[kPlanThreads / 32][2];
-  int *start = plan_smem, *first = plan_smem + B + 1;
-  const int t = threadIdx.x, count = min(max(*free_count, 0), F);
+  __shared__ long long warps[3][32];
+  int *start = plan_smem, *first = start + B + 1, *length = first + B + 1;
+  const int t = threadIdx.x, threads = blockDim.x, have = *free_count;
   long long tokens = 0, pages = 0, wanted = 0;
-  for (int base = 0; base < B; base += kPlanThreads) {
-    const int b = base + t;
-    const int len = b < B ? max(lengths[b], 0) : 0;
-    long long n = b < B ? max(add[b], 0) : 0, zero = 0, all, none;
-    const long long mine = n;
-    scan2(n, zero, all, none, warps);
-    const long long lo = min(tokens + n, static_cast<long long>(N)), hi = min(tokens + n + mine, static_cast<long long>(N));
+  for (int base = 0; base < B; base += threads) {
+    const int b = base + t, len = b < B ? max(lengths[b], 0) : 0;
+    const long long mine = b < B ? max(add[b], 0) : 0;
+    long long all, all_take, all_lack;
+    const long long from = tokens + scan(mine, all, warps[0]);
+    const long long lo = min(from, static_cast<long long>(N)), hi = min(from + mine, static_cast<long long>(N));
     const int held = pages_for(len, shift), need = pages_for(len + (hi - lo), shift);
-    long long take = min(need, W) - min(held, W), lack = need - held, all_take, all_lack;
-    scan2(take, lack, all_take, all_lack, warps);
+    const long long take = min(need, W) - min(held, W), lack = need - held;
+    const long long before = pages + scan(take, all_take, warps[1]);
+    scan(lack, all_lack, warps[2]);
     if (b < B) {
       start[b] = static_cast<int>(lo);
-      first[b] = static_cast<int>(pages + take);
+      first[b] = static_cast<int>(before);
+      length[b] = len;
       if (blockIdx.x == 0) {
         query_start[b] = static_cast<int>(lo);
         total[b] = static_cast<int>(len + (hi - lo));
@@ -68,7 +72,9 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const int* __r
     tokens += all;
     pages += all_take;
     wanted += all_lack;
+    if (base + threads < B) __syncthreads();                           // the sums have been read
   }
+  const int count = min(max(have, 0), F);
   if (t == 0) {
     start[B] = static_cast<int>(min(tokens, static_cast<long long>(N)));
     first[B] = static_cast<int>(pages);
@@ -80,29 +86,30 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const int* __r
     }
   }
   __syncthreads();
-  const int lane = t & 31, warp = blockIdx.x * (kPlanThreads / 32) + (t >> 5), warps_all = gridDim.x * (kPlanThreads / 32);
-  for (int b = warp; b < B; b += warps_all) {
-    const int held = pages_for(max(lengths[b], 0), shift), n = first[b + 1] - first[b];
-    for (int j = lane; j < n; j += 32) {
-      const int order = first[b] + j;
-      table[static_cast<long>(b) * W + held + j] = order < count ? free_pages[count - 1 - order] : -1;
+  // new entries: entry `order` belongs to the last request whose first one is not behind it
+  auto find = [&](const int* from, long long what) {
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (from[mid] <= what) lo = mid; else hi = mid;
     }
+    return lo;
+  };
+  const int step = gridDim.x * threads, me = blockIdx.x * threads + t;
+  for (long long order = me; order < pages; order += step) {
+    const int b = find(first, order);
+    table[static_cast<long>(b) * W + pages_for(length[b], shift) + (order - first[b])] = order < count ? free_pages[count - 1 - order] : -1;
   }
-  for (long i = static_cast<long>(blockIdx.x) * kPlanThreads + t; i < N; i += static_cast<long>(gridDim.x) * kPlanThreads) {
+  for (long long i = me; i < N; i += step) {
     long long slot = -1, pos = 0;
     if (i < start[B]) {
-      int lo = 0, hi = B;                       // the last request that begins at i or before and is not empty
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (start[mid] <= i) lo = mid; else hi = mid;
-      }
-      const int len = max(lengths[lo], 0), held = pages_for(len, shift);
-      pos = len + (i - start[lo]);
+      const int b = find(start, i), len = length[b], held = pages_for(len, shift);
+      pos = len + (i - start[b]);
       const long long j = pos >> shift;
       int page = -1;
       if (j < W) {
-        const long long order = first[lo] + (j - held);
-        page = j < held ? table[static_cast<long>(lo) * W + j] : order < count ? free_pages[count - 1 - order] : -1;
+        const long long order = first[b] + (j - held);
+        page = j < held ? table[static_cast<long>(b) * W + j] : order < count ? free_pages[count - 1 - order] : -1;
       }
       if (page >= 0) slot = (static_cast<long long>(page) << shift) + (pos & ((1 << shift) - 1));
     }
@@ -117,7 +124,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_release_kernel(const uint8
                                                                      const int* __restrict__ free_count, int F, int* __restrict__ total,
                                                                      int* __restrict__ free_left, int B, int W, int shift) {
   __shared__ int have[kPlanThreads];
-  __shared__ long long warps[kPlanThreads / 32][2];
+  __shared__ long long warps[32];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   long long at = min(max(*free_count, 0), F);
   for (int base = 0; base < B; base += kPlanThreads) {
@@ -133,9 +140,9 @@ __global__ void __launch_bounds__(kPlanThreads) cache_release_kernel(const uint8
       if (lane == 0) have[i] = n;
     }
     __syncthreads();
-    long long mine = t < end ? have[t] : 0, zero = 0, all, none;
-    scan2(mine, zero, all, none, warps);
-    if (t < end) have[t] = static_cast<int>(mine);
+    long long all;
+    const long long before = scan(static_cast<long long>(t < end ? have[t] : 0), all, warps);
+    if (t < end) have[t] = static_cast<int>(before);
     __syncthreads();
     for (int i = warp; i < end; i += kPlanThreads / 32) {
       const int b = base + i;
@@ -174,91 +181,231 @@ __device__ __forceinline__ int exponent_of(float scale) {
   const int e = static_cast<int>(__float_as_uint(scale) >> 23) - 127;
   return e > kMaxExp ? kNoStep : max(e, kMinExp);
 }
-__device__ __forceinline__ uint8_t code_of(float x, float inv) { return static_cast<uint8_t>(static_cast<int>(rintf(x * inv)) + 128); }
+// 128 + x * step, rounded to the nearest whole number (half to even), in the low byte: 1.5 * 2^23 leaves no bits behind the point
+__device__ __forceinline__ uint32_t code_of(float x, float step) { return __float_as_uint(fmaf(x, step, 12583040.f)); }
+__device__ __forceinline__ uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// Codes of one byte each on the grid that is `ratio` times coarser
+__device__ __forceinline__ uint32_t coarser(uint32_t w, float ratio) {
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = code_of(static_cast<float>(w >> (8 * i) & 0xff) - 128.f, ratio);
+  return bytes4(c[0], c[1], c[2], c[3]);
+}
 
-constexpr int kAppendThreads = 128;
+// The last request that begins at i or before, by a warp: 32 requests a load
+__device__ __forceinline__ int request_at(const int* start, int B, int i) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, size = B;
+  while (size > 32) {
+    const int step = (size + 31) / 32, at = lo + lane * step;
+    const int n = __popc(__ballot_sync(0xffffffffu, at < lo + size && start[at] <= i));
+    lo += max(n - 1, 0) * step;
+    size = min(step, B - lo);
+  }
+  return lo + max(__popc(__ballot_sync(0xffffffffu, lane < size && start[lo + lane] <= i)) - 1, 0);
+}
 
-// One CTA per window of packed tokens and head.  The tokens of a request that lie in one page are a group, handled by the CTA
-// in whose window the first of them lies: their largest magnitudes give the page's scales, codes that are there are rounded again where
-// a scale grows, then the new ones are stored.
-__global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long ldk, long ldv, CachePages c,
-                                                                      CacheStep s, int window) {
-  __shared__ unsigned red[kAppendThreads / 32][2];
-  const int h = blockIdx.y, t = threadIdx.x, D = c.D, P = 1 << c.shift;
-  const int total = min(s.query_start[s.B], s.N);
-  int i = blockIdx.x * window;
-  const int end = min(i + window, total);
-  while (i < end) {
-    int lo = 0, hi = s.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s.query_start[mid] <= i) lo = mid; else hi = mid;
+// One CTA per window of packed tokens, head and side.  The tokens of a request that lie in one page are a group, handled by the CTA in whose window the
+// first of them lies: their largest magnitude gives the page's scale, codes that are there are rounded again where it grows, then the new ones are
+// stored.  A warp takes 16 tokens of 32 * C columns at a time, a lane C columns of them, so that it reads whole rows of 64 or 128 columns, its 16 tokens are
+// 16 bytes of each column of the values, and what it holds in registers between the maximum and the codes is read once (one such block; pages of
+// 256 tokens with more than 128 columns read the rest again).  Bytes bound it.  XX
+template <int C>
+struct Block {                             // 16 tokens, C columns of a lane
+  uint32_t w[16][C / 2];
+};
+template <int C>
+__device__ __forceinline__ void load_block(Block<C>& x, const bf16* src, long ld, int t0, int from, int to) {   // tokens from .. to of t0 .. t0 + 15
+#pragma unroll
+  for (int t = 0; t < 16; ++t) {
+    const bool in = t0 + t >= from && t0 + t < to;
+    if (C == 4) {
+      const uint2 v = in ? *reinterpret_cast<const uint2*>(src + (t0 + t - from) * ld) : make_uint2(0, 0);
+      x.w[t][0] = v.x;
+      x.w[t][C / 2 - 1] = v.y;
+    } else {
+      x.w[t][0] = in ? *reinterpret_cast<const uint32_t*>(src + (t0 + t - from) * ld) : 0u;
     }
-    const int first = s.query_start[lo], last = min(s.query_start[lo + 1], total);
-    const long pos = static_cast<long>(s.lengths[lo]) - s.query_start[lo + 1] + i;
-    const int off = static_cast<int>(pos & (P - 1));
-    const int m = max(min(last - i, P - off), 1);
-    const int page = page_of(s, c, lo, pos);
-    if ((off != 0 && i != first) || page < 0) {
-      i += m;
+  }
+}
+template <int C>
+__device__ __forceinline__ unsigned amax_of(const Block<C>& x) {
+  unsigned m = 0;                          // magnitudes as bits, two 16-bit numbers at a time: NaN above infinity above all numbers
+#pragma unroll
+  for (int t = 0; t < 16; ++t)
+#pragma unroll
+    for (int c = 0; c < C / 2; ++c) m = __vmaxu2(m, x.w[t][c] & 0x7fff7fffu);
+  return max(m << 16, m & 0xffff0000u);
+}
+// Codes of a block, and of what is in its place: tokens before `from` are rounded to a grid coarser by `ratio` (1: left), from .. to are new.
+template <int C>
+__device__ __forceinline__ void store_keys(uint8_t* codes, const Block<C>& x, int D, int d, int t0, int from, int to, float ratio, float inv, bool bad) {
+#pragma unroll
+  for (int t = 0; t < 16; ++t) {
+    const int tok = t0 + t;
+    uint8_t* at = codes + key_at(tok, d, D);
+    uint32_t w = 0x80808080u;
+    if (tok >= from && tok < to) {
+      if (!bad) {
+        const uint32_t a = code_of(low(x.w[t][0]), inv), b = code_of(high(x.w[t][0]), inv);
+        w = bytes4(a, b, C == 4 ? code_of(low(x.w[t][C / 2 - 1]), inv) : 0, C == 4 ? code_of(high(x.w[t][C / 2 - 1]), inv) : 0);
+      }
+    } else if (tok < from && ratio != 1.f) {
+      w = coarser(C == 4 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at), ratio);
+    } else {
       continue;
     }
-    unsigned ak = 0, av = 0;                     // magnitudes as bits: NaN above infinity above all numbers
-    for (int x = t; x < m * D; x += kAppendThreads) {
-      const long r = i + x / D;
-      const int d = x % D;
-      ak = max(ak, __float_as_uint(__bfloat162float(k[r * ldk + h * D + d])) & 0x7fffffffu);
-      av = max(av, __float_as_uint(__bfloat162float(v[r * ldv + h * D + d])) & 0x7fffffffu);
+    if (C == 4) *reinterpret_cast<uint32_t*>(at) = w;
+    else *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(w);
+  }
+}
+template <int C>
+__device__ __forceinline__ void store_values(uint8_t* codes, const Block<C>& x, int D, int d, int t0, int from, int to, float ratio, float inv, bool bad) {
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    uint4* at = reinterpret_cast<uint4*>(codes + value_at(t0, d + c, D));
+    uint32_t w[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+    if (t0 < from || t0 + 16 > to) {                                   // some of the 16 are others
+      const uint4 v = *at;
+      w[0] = v.x;
+      w[1] = v.y;
+      w[2] = v.z;
+      w[3] = v.w;
     }
-    for (int o = 16; o; o >>= 1) {
-      ak = max(ak, __shfl_xor_sync(0xffffffffu, ak, o));
-      av = max(av, __shfl_xor_sync(0xffffffffu, av, o));
-    }
-    if ((t & 31) == 0) { red[t >> 5][0] = ak; red[t >> 5][1] = av; }
-    __syncthreads();
-    for (int w = 0; w < kAppendThreads / 32; ++w) { ak = max(ak, red[w][0]); av = max(av, red[w][1]); }
-    const long ph = static_cast<long>(page) * c.H + h;
-    int e[2] = {step_exponent(ak), step_exponent(av)}, old[2] = {e[0], e[1]};
-    if (off)
-      for (int x = 0; x < 2; ++x) {
-        old[x] = exponent_of(c.scale[ph * 2 + x]);
-        e[x] = max(e[x], old[x]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t n[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t v = x.w[4 * q + i][c / 2];
+        n[i] = bad ? 128u : code_of(c & 1 ? high(v) : low(v), inv);
       }
-    __syncthreads();                             // the scales have been read
-    uint8_t *kc = c.k + ph * P * D, *vc = c.v + ph * P * D;
-    for (int x = 0; x < 2; ++x) {
-      uint8_t* codes = x ? vc : kc;
-      if (e[x] != old[x] && e[x] != kNoStep) {
-        const float ratio = power2(max(old[x] - e[x], -126));
-        for (int y = t; y < off * D; y += kAppendThreads) {
-          const int at = x ? value_at(y / D, y % D, D) : key_at(y / D, y % D, D);
-          codes[at] = code_of(static_cast<float>(codes[at]) - 128.f, ratio);
-        }
-      }
-      const float inv = e[x] == kNoStep ? 0.f : power2(-e[x]);
-      for (int y = t; y < m * D; y += kAppendThreads) {
-        const long r = i + y / D;
-        const int d = y % D, tok = off + y / D;
-        const float f = __bfloat162float(x ? v[r * ldv + h * D + d] : k[r * ldk + h * D + d]);
-        codes[x ? value_at(tok, d, D) : key_at(tok, d, D)] = e[x] == kNoStep ? 128 : code_of(f, inv);
+      const uint32_t fresh = bytes4(n[0], n[1], n[2], n[3]), old = ratio != 1.f ? coarser(w[q], ratio) : w[q];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = t0 + 4 * q + i;
+        const uint32_t byte = 0xffu << (8 * i);
+        w[q] = tok >= to ? w[q] : (w[q] & ~byte) | ((tok >= from ? fresh : old) & byte);
       }
     }
-    if (t < 2) c.scale[ph * 2 + t] = e[t] == kNoStep ? __int_as_float(0x7fc00000) : power2(e[t]);
-    i += m;
+    *at = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
-// One CTA per page and head: bf16 values (n, P, H, D) of both sides.
+template <int C>
+__global__ void __launch_bounds__(512) cache_append_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long ldk, long ldv, CachePages c, CacheStep s,
+                                                           int window) {
+  __shared__ unsigned red[16];
+  const int h = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5, D = c.D, P = 1 << c.shift;
+  const bool values = blockIdx.z;
+  const bf16* x = (values ? v : k) + h * D;
+  const long ld = values ? ldv : ldk;
+  const int total = min(s.query_start[s.B], s.N), slabs = D / (32 * C);
+  int i = blockIdx.x * window;
+  const int end = min(i + window, total);
+  while (i < end) {
+    const int b = request_at(s.query_start, s.B, i), first = s.query_start[b], next = s.query_start[b + 1];
+    const long pos = static_cast<long>(s.lengths[b]) - next + i;
+    const int off = static_cast<int>(pos & (P - 1)), m = max(min(min(next, total) - i, P - off), 1);
+    if (off != 0 && i != first) {                                      // of a group that began in another window
+      i += m;
+      continue;
+    }
+    // blocks of the group: 16 tokens each from off / 16 on, by columns
+    const int g0 = off >> 4, blocks = (((off + m - 1) >> 4) - g0 + 1) * slabs;
+    const bf16* src = x + static_cast<long>(i) * ld;
+    Block<C> held;
+    unsigned top = 0;
+    auto get = [&](int y) { load_block(held, src + (y % slabs) * 32 * C + lane * C, ld, (g0 + y / slabs) * 16, off, off + m); };
+    for (int y = warp + warps; y < blocks; y += warps) {
+      get(y);
+      top = max(top, amax_of(held));
+    }
+    if (warp < blocks) {
+      get(warp);
+      top = max(top, amax_of(held));
+    }
+    const int page = page_of(s, c, b, pos);
+    const long ph = static_cast<long>(max(page, 0)) * c.H + h;
+    const float before = c.scale[ph * 2 + values];
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+    for (int w = 0; w < warps; ++w) top = max(top, red[w]);
+    i += m;
+    __syncthreads();                                                   // the maxima have been read; and the scale
+    if (page < 0) continue;
+    int e = step_exponent(top), old = e;
+    if (off) {
+      old = exponent_of(before);
+      e = max(e, old);
+    }
+    const bool bad = e == kNoStep;
+    const float inv = bad ? 0.f : power2(-e), ratio = bad ? 1.f : power2(max(old - e, -126));
+    uint8_t* codes = (values ? c.v : c.k) + ph * P * D;
+    for (int y = warp; y < blocks; y += warps) {
+      if (y != warp) get(y);
+      const int d = (y % slabs) * 32 * C + lane * C, t0 = (g0 + y / slabs) * 16;
+      if (values) store_values(codes, held, D, d, t0, off, off + m, ratio, inv, bad);
+      else store_keys(codes, held, D, d, t0, off, off + m, ratio, inv, bad);
+    }
+    if (ratio != 1.f)                                                  // all codes before the group's blocks: bytes, whatever their order
+      for (int y = t * 16; y < g0 * 16 * D; y += blockDim.x * 16) {
+        uint4* at = reinterpret_cast<uint4*>(codes + y);
+        const uint4 w = *at;
+        *at = make_uint4(coarser(w.x, ratio), coarser(w.y, ratio), coarser(w.z, ratio), coarser(w.w, ratio));
+      }
+    if (t == 0) c.scale[ph * 2 + values] = bad ? __int_as_float(0x7fc00000) : power2(e);
+  }
+}
+
+// One CTA per page and head: bf16 values (n, P, H, D) of both sides.  Keys 16 codes of a token at a time; values 16 tokens of C columns, so that a warp's
+// stores are whole rows.  Bytes bound it.  XX
+template <int C>
 __global__ void __launch_bounds__(128) cache_values_kernel(CachePages c, const int* __restrict__ ids, bf16* __restrict__ k, bf16* __restrict__ v) {
-  const int h = blockIdx.y, P = 1 << c.shift, D = c.D, page = ids[blockIdx.x];
+  const int h = blockIdx.y, P = 1 << c.shift, D = c.D, page = ids[blockIdx.x], t = threadIdx.x, lane = t & 31;
   const bool there = page >= 0 && page < c.pages;
-  const long ph = static_cast<long>(there ? page : 0) * c.H + h;
-  const float sk = c.scale[ph * 2], sv = c.scale[ph * 2 + 1];
-  for (int x = threadIdx.x; x < P * D; x += 128) {
-    const int tok = x / D, d = x % D;
-    const long at = ((static_cast<long>(blockIdx.x) * P + tok) * c.H + h) * D + d;
-    k[at] = __float2bfloat16(there ? (c.k[ph * P * D + key_at(tok, d, D)] - 128.f) * sk : 0.f);
-    v[at] = __float2bfloat16(there ? (c.v[ph * P * D + value_at(tok, d, D)] - 128.f) * sv : 0.f);
+  const long ph = static_cast<long>(there ? page : 0) * c.H + h, row = static_cast<long>(c.H) * D, out = static_cast<long>(blockIdx.x) * P * row + h * D;
+  const float2 scale = *reinterpret_cast<const float2*>(c.scale + ph * 2);
+  auto two = [](uint32_t w, int i, float s) {                          // codes i and i + 1 of a word
+    const __nv_bfloat162 r = __floats2bfloat162_rn((static_cast<float>(w >> (8 * i) & 0xff) - 128.f) * s, (static_cast<float>(w >> (8 * i + 8) & 0xff) - 128.f) * s);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  };
+  const uint8_t* kc = c.k + ph * P * D;
+  for (int y = t * 16; y < P * D; y += 128 * 16) {
+    const int token = y / (2 * D) * 2 + (y >> 6 & 1), d = (y % (2 * D) >> 7) * 64 + (y & 63);
+    const uint4 w = there ? *reinterpret_cast<const uint4*>(kc + y) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+    const float s = there ? scale.x : 0.f;
+    uint4* to = reinterpret_cast<uint4*>(k + out + token * row + d);
+    to[0] = make_uint4(two(w.x, 0, s), two(w.x, 2, s), two(w.y, 0, s), two(w.y, 2, s));
+    to[1] = make_uint4(two(w.z, 0, s), two(w.z, 2, s), two(w.w, 0, s), two(w.w, 2, s));
+  }
+  const uint8_t* vc = c.v + ph * P * D;
+  const int slabs = D / (32 * C);
+  const float s = there ? scale.y : 0.f;
+  for (int y = t >> 5; y < P / 16 * slabs; y += 4) {
+    const int t0 = y / slabs * 16, d = (y % slabs) * 32 * C + lane * C;
+    uint32_t w[C][4];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const uint4 u = there ? *reinterpret_cast<const uint4*>(vc + value_at(t0, d + i, D)) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+      w[i][0] = u.x;
+      w[i][1] = u.y;
+      w[i][2] = u.z;
+      w[i][3] = u.w;
+    }
+    auto number = [&](int i, int tok) { return (static_cast<float>(w[i][tok >> 2] >> (8 * (tok & 3)) & 0xff) - 128.f) * s; };
+#pragma unroll
+    for (int tok = 0; tok < 16; ++tok) {
+      bf16* to = v + out + (t0 + tok) * row + d;
+      const __nv_bfloat162 a = __floats2bfloat162_rn(number(0, tok), number(1, tok)), b = __floats2bfloat162_rn(number(C - 2, tok), number(C - 1, tok));
+      if (C == 4) *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      else *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(&a);
+    }
   }
 }
 }  // namespace
@@ -268,14 +415,15 @@ extern "C" int nsa_cache_plan(const int* lengths, const int* add, int* table, co
                               int page_size, cudaStream_t st) {
   if (B <= 0 || W <= 0 || N < 0 || F < 0) return nsa::fail(NSA_ERR_SHAPE, "cache_plan: empty problem");
   if (B > nsa_cache_plan_limit()) return nsa::fail(NSA_ERR_LIMIT, "cache_plan: more requests than shared memory holds");
-  const int bytes = 2 * (B + 1) * 4;
+  const int bytes = 3 * (B + 1) * 4;
   if (bytes > 40000) {
     const cudaError_t e = cudaFuncSetAttribute(cache_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200000);
     if (e != cudaSuccess) return nsa::fail_cuda(e, "nsa_cache_plan");
   }
-  const int want = (N + 4 * kPlanThreads - 1) / (4 * kPlanThreads), most = nsa::sm_count();
+  const int threads = B <= 128 ? 128 : B <= 512 ? 512 : kPlanThreads;
+  const int want = (N + threads - 1) / threads, most = nsa::sm_count();
   const int grid = want < 1 ? 1 : want < most ? want : most;
-  cache_plan_kernel<<<grid, kPlanThreads, bytes, st>>>(lengths, add, table, free_pages, free_count, F, query_start, total, slots, positions, free_left,
+  cache_plan_kernel<<<grid, threads, bytes, st>>>(lengths, add, table, free_pages, free_count, F, query_start, total, slots, positions, free_left,
                                                        shortfall, B, W, N, __builtin_ctz(page_size));
   nsa::count_launch();
   const cudaError_t e = cudaGetLastError();
@@ -300,9 +448,14 @@ extern "C" int nsa_cache_append(const void* k, const void* v, long ldk, long ldv
   if (B <= 0 || H <= 0 || H > 65535 || D % 64 || N < 0) return nsa::fail(NSA_ERR_SHAPE, "cache_append: unsupported shape");
   const CachePages c{static_cast<uint8_t*>(kc), static_cast<uint8_t*>(vc), scale, pages, H, D, __builtin_ctz(page_size)};
   const CacheStep s{table, query_start, lengths, B, W, N};
-  const int window = N <= 2048 ? 1 : page_size;
-  cache_append_kernel<<<dim3((N + window - 1) / window, H), kAppendThreads, 0, st>>>(static_cast<const bf16*>(k), static_cast<const bf16*>(v), ldk, ldv, c, s,
-                                                                                     window);
+  // few tokens: one a CTA, most of them the first of their page; else a page's worth.  Warps for the 16-token blocks of a page
+  const int window = N <= 2048 ? 1 : page_size, C = D % 128 ? 2 : 4, blocks = page_size / 16 * (D / (32 * C));
+  const int warps = window == 1 && N <= B ? 1 : blocks < 16 ? blocks : 16;
+  const dim3 grid((N + window - 1) / window, H, 2);
+  if (C == 4)
+    cache_append_kernel<4><<<grid, 32 * warps, 0, st>>>(static_cast<const bf16*>(k), static_cast<const bf16*>(v), ldk, ldv, c, s, window);
+  else
+    cache_append_kernel<2><<<grid, 32 * warps, 0, st>>>(static_cast<const bf16*>(k), static_cast<const bf16*>(v), ldk, ldv, c, s, window);
   nsa::count_launch();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : nsa::fail_cuda(e, "nsa_cache_append launch");
@@ -314,7 +467,10 @@ extern "C" int nsa_cache_values(const void* kc, const void* vc, const float* sca
   if (H <= 0 || H > 65535 || D % 64 || n < 0) return nsa::fail(NSA_ERR_SHAPE, "cache_values: unsupported shape");
   const CachePages c{static_cast<uint8_t*>(const_cast<void*>(kc)), static_cast<uint8_t*>(const_cast<void*>(vc)), const_cast<float*>(scale), pages, H, D,
                      __builtin_ctz(page_size)};
-  cache_values_kernel<<<dim3(n, H), 128, 0, st>>>(c, ids, static_cast<bf16*>(k), static_cast<bf16*>(v));
+  if (D % 128)
+    cache_values_kernel<2><<<dim3(n, H), 128, 0, st>>>(c, ids, static_cast<bf16*>(k), static_cast<bf16*>(v));
+  else
+    cache_values_kernel<4><<<dim3(n, H), 128, 0, st>>>(c, ids, static_cast<bf16*>(k), static_cast<bf16*>(v));
   nsa::count_launch();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : nsa::fail_cuda(e, "nsa_cache_values launch");
