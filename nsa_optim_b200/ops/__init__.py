@@ -275,7 +275,7 @@ def cache_pages(pages: int, heads: int, head_dim: int, page_size: int = 64, devi
 
 def _cache_native(t: Tensor) -> bool:
     """Whether the cache's ops on tensors of whole numbers run as kernels."""
-    return t.is_cuda and _BACKEND != "torch" and native_module() is not None
+    return t.is_cuda and _BACKEND != "torch" and (_native is not None or native_module() is not None)
 
 
 def cache_plan(lengths: Tensor, new: Tensor, table: Tensor, free: Tensor, free_count: Tensor, num_tokens: int,

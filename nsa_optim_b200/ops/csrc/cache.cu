@@ -218,17 +218,18 @@ template <int C>
 struct Block {                             // 16 tokens, C columns of a lane
   uint32_t w[16][C / 2];
 };
-template <int C>
-__device__ __forceinline__ void load_block(Block<C>& x, const bf16* src, long ld, int t0, int from, int to) {   // tokens from .. to of t0 .. t0 + 15
+// Tokens from .. to of t0 .. t0 + 15; FULL: all of them.  src: token t0's row, which may lie outside.
+template <int C, bool FULL>
+__device__ __forceinline__ void load_block(Block<C>& x, const bf16* src, long ld, int t0, int from, int to) {
 #pragma unroll
   for (int t = 0; t < 16; ++t) {
-    const bool in = t0 + t >= from && t0 + t < to;
+    const bool in = FULL || (t0 + t >= from && t0 + t < to);
     if (C == 4) {
-      const uint2 v = in ? *reinterpret_cast<const uint2*>(src + (t0 + t - from) * ld) : make_uint2(0, 0);
+      const uint2 v = in ? __ldcs(reinterpret_cast<const uint2*>(src + t * ld)) : make_uint2(0, 0);
       x.w[t][0] = v.x;
       x.w[t][C / 2 - 1] = v.y;
     } else {
-      x.w[t][0] = in ? *reinterpret_cast<const uint32_t*>(src + (t0 + t - from) * ld) : 0u;
+      x.w[t][0] = in ? __ldcs(reinterpret_cast<const uint32_t*>(src + t * ld)) : 0u;
     }
   }
 }
@@ -240,6 +241,36 @@ __device__ __forceinline__ unsigned amax_of(const Block<C>& x) {
 #pragma unroll
     for (int c = 0; c < C / 2; ++c) m = __vmaxu2(m, x.w[t][c] & 0x7fff7fffu);
   return max(m << 16, m & 0xffff0000u);
+}
+// Codes of a block whose 16 tokens are all new
+template <int C>
+__device__ __forceinline__ void store_full(uint8_t* codes, const Block<C>& x, bool values, int D, int d, int t0, float inv) {
+  if (values) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      uint32_t w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t n[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t v = x.w[4 * q + i][c / 2];
+          n[i] = code_of(c & 1 ? high(v) : low(v), inv);
+        }
+        w[q] = bytes4(n[0], n[1], n[2], n[3]);
+      }
+      *reinterpret_cast<uint4*>(codes + value_at(t0, d + c, D)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+    uint8_t* at = codes + key_at(t0, d, D);
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      const uint32_t a = code_of(low(x.w[t][0]), inv), b = code_of(high(x.w[t][0]), inv);
+      uint8_t* to = at + (t >> 1) * 2 * D + (t & 1) * 64;
+      if (C == 4) *reinterpret_cast<uint32_t*>(to) = bytes4(a, b, code_of(low(x.w[t][C / 2 - 1]), inv), code_of(high(x.w[t][C / 2 - 1]), inv));
+      else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(__byte_perm(a, b, 0x0040));
+    }
+  }
 }
 // Codes of a block, and of what is in its place: tokens before `from` are rounded to a grid coarser by `ratio` (1: left), from .. to are new.
 template <int C>
@@ -297,7 +328,7 @@ __device__ __forceinline__ void store_values(uint8_t* codes, const Block<C>& x, 
 }
 
 template <int C>
-__global__ void __launch_bounds__(512) cache_append_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long ldk, long ldv, CachePages c, CacheStep s,
+__global__ void __maxnreg__(80) cache_append_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long ldk, long ldv, CachePages c, CacheStep s,
                                                            int window) {
   __shared__ unsigned red[16];
   const int h = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5, D = c.D, P = 1 << c.shift;
@@ -320,7 +351,13 @@ __global__ void __launch_bounds__(512) cache_append_kernel(const bf16* __restric
     const bf16* src = x + static_cast<long>(i) * ld;
     Block<C> held;
     unsigned top = 0;
-    auto get = [&](int y) { load_block(held, src + (y % slabs) * 32 * C + lane * C, ld, (g0 + y / slabs) * 16, off, off + m); };
+    auto full = [&](int t0) { return t0 >= off && t0 + 16 <= off + m; };
+    auto get = [&](int y) {
+      const int t0 = (g0 + y / slabs) * 16;
+      const bf16* row = src + (t0 - off) * ld + (y % slabs) * 32 * C + lane * C;
+      if (full(t0)) load_block<C, true>(held, row, ld, t0, off, off + m);
+      else load_block<C, false>(held, row, ld, t0, off, off + m);
+    };
     for (int y = warp + warps; y < blocks; y += warps) {
       get(y);
       top = max(top, amax_of(held));
@@ -350,7 +387,8 @@ __global__ void __launch_bounds__(512) cache_append_kernel(const bf16* __restric
     for (int y = warp; y < blocks; y += warps) {
       if (y != warp) get(y);
       const int d = (y % slabs) * 32 * C + lane * C, t0 = (g0 + y / slabs) * 16;
-      if (values) store_values(codes, held, D, d, t0, off, off + m, ratio, inv, bad);
+      if (full(t0) && !bad) store_full(codes, held, values, D, d, t0, inv);
+      else if (values) store_values(codes, held, D, d, t0, off, off + m, ratio, inv, bad);
       else store_keys(codes, held, D, d, t0, off, off + m, ratio, inv, bad);
     }
     if (ratio != 1.f)                                                  // all codes before the group's blocks: bytes, whatever their order

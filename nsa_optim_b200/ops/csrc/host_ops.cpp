@@ -1180,6 +1180,14 @@ Tensor packed_rows(const Tensor& t) {
   return ok ? t : at::empty(t.sizes(), t.options()).copy_(t);
 }
 
+// n numbers of `base`, a row of bytes, from `at` on: what as_strided does, without the dispatcher (1 us each)
+Tensor slice(const Tensor& base, at::ScalarType dtype, int64_t at, int64_t n) {
+  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(dtype));
+  t.unsafeGetTensorImpl()->set_storage_offset(base.storage_offset() / static_cast<int64_t>(c10::elementSize(dtype)) + at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(n);
+  return t;
+}
+
 OP(cache_plan) {                                 // lengths, new, table, free, free_count, tokens, page size -> the fields of a CachePlan
   return entry(py, np, [](Args& a) {
     const Tensor &lengths = a.t(), &add = a.t(), &table = a.t(), &pages = a.t(), &count = a.t();
@@ -1197,8 +1205,20 @@ OP(cache_plan) {                                 // lengths, new, table, free, f
       WANT(count.size(0) == 1 && N >= 0, "free_count has one element, num_tokens is not negative");
       want_dense(table, "table");
       const Tensor l = lengths.contiguous(), n = add.contiguous(), f = pages.contiguous();
-      const Tensor start = alloc({B + 1}, I32, dev), total = alloc({B}, I32, dev), slots = alloc({N}, I64, dev), at = alloc({N}, I64, dev);
-      const Tensor left = alloc({1}, I32, dev), lack = alloc({1}, I32, dev);
+      // one allocation for the six results; with guard zones on, one each
+      Tensor start, total, slots, at, left, lack;
+      if (t_guarded) {
+        start = alloc({B + 1}, I32, dev), total = alloc({B}, I32, dev), slots = alloc({N}, I64, dev), at = alloc({N}, I64, dev);
+        left = alloc({1}, I32, dev), lack = alloc({1}, I32, dev);
+      } else {
+        const Tensor all = alloc({16 * N + 4 * (2 * B + 3)}, at::kByte, dev);
+        slots = slice(all, I64, 0, N);
+        at = slice(all, I64, N, N);
+        start = slice(all, I32, 4 * N, B + 1);
+        total = slice(all, I32, 4 * N + B + 1, B);
+        left = slice(all, I32, 4 * N + 2 * B + 1, 1);
+        lack = slice(all, I32, 4 * N + 2 * B + 2, 1);
+      }
       launch(lib.nsa_cache_plan, ip(l), ip(n), ip(table), ip(f), ip(count), small(f.numel(), "the stack"), ip(start), ip(total), lp(slots), lp(at),
              ip(left), ip(lack), small(B, "the number of requests"), small(W, "table"), small(N, "num_tokens"), dim(P));
       return {start, total, slots, at, left, lack};

@@ -1218,7 +1218,7 @@ def _ssd_scan_batched(x, dt, A, Bm, Cm, D=None, chunk=256):
 # generation and scoring (csrc/cache.cu, csrc/cache_attention.cu, csrc/logprobs.cu)
 # --------------------------------------------------------------------------------------
 def cache_plan(lengths, new, table, free, free_count, num_tokens, page_size):
-    if lengths.shape[:1].numel() > 16384:                      # one CTA holds a number for each request
+    if lengths.dim() == 1 and lengths.shape[0] > 16384:        # a CTA holds three numbers for each request
         _fallback("cache_plan")
         return cache.plan(lengths, new, table, free, free_count, num_tokens, page_size)
     return cache.CachePlan(*_h().cache_plan(lengths, new, table, free, free_count, num_tokens, page_size))
