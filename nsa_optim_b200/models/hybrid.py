@@ -213,13 +213,15 @@ class HybridModel(CausalLMBase):
                 nn.init.normal_(mod.weight, mean=0.0, std=std)
 
     def forward(self, input_ids: Tensor, attention_mask: Optional[Tensor] = None,
-                labels: Optional[Tensor] = None, position_ids: Optional[Tensor] = None, **_):
+                labels: Optional[Tensor] = None, position_ids: Optional[Tensor] = None, return_hidden: bool = False, **_):
         # without position_ids the rotary tables are sliced by length: explicit ids cost each attention block a
         # device synchronisation (their maximum) and two gathers
         h = self.embed_tokens(input_ids)
         for layer in self.layers:
             h = self.run_layer(layer, h, attention_mask, position_ids)
         h = self.norm(h)
+        if return_hidden:                                    # what the output head is applied to
+            return h, None, None
         logits, loss = self.compute_loss(h, labels)
         return logits, loss, None
 

@@ -116,6 +116,12 @@ class RotaryEmbedding(nn.Module):
         self.cos_cached, self.sin_cached = cos, sin
         self.max_seq_len_cached = seq_len
 
+    def rows(self, positions: Tensor, limit: int) -> Tuple[Tensor, Tensor]:
+        """The rows of positions below ``limit``, a number that the host knows, so that it does not wait for their maximum."""
+        if limit > self.max_seq_len_cached or self.cos_cached.device != positions.device:
+            self._set_cos_sin_cache(max(limit, self._initial), device=positions.device)
+        return self.cos_cached[positions], self.sin_cached[positions]
+
     def forward(self, x: Tensor, position_ids: Optional[Tensor] = None, seq_len: Optional[int] = None
                 ) -> Tuple[Tensor, Tensor]:
         need = int(position_ids.max()) + 1 if position_ids is not None else (seq_len or x.shape[1])

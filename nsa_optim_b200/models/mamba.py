@@ -129,11 +129,13 @@ class _SSMModel(CausalLMBase):
             blk.apply(init_linear_embedding_)
 
     def forward(self, input_ids: Tensor, attention_mask: Optional[Tensor] = None,
-                labels: Optional[Tensor] = None, **_):
+                labels: Optional[Tensor] = None, return_hidden: bool = False, **_):
         h = self.embed_tokens(input_ids)
         for layer in self.layers:
             h = self.run_layer(layer, h)
         h = self.norm(h)
+        if return_hidden:                                    # what the output head is applied to
+            return h, None, None
         logits, loss = self.compute_loss(h, labels)
         return logits, loss, None
 

@@ -58,20 +58,26 @@ class DenseAttention(nn.Module):
         self.o_proj = Linear(self.num_heads * self.head_dim, self.hidden_size)
         self.rotary_emb = RotaryEmbedding(self.head_dim, config.max_position_embeddings, config.rope_theta)
 
-    def _qkv(self, x: Tensor, position_ids: Optional[Tensor]):
+    def _qkv(self, x: Tensor, position_ids: Optional[Tensor], rotary=None):
         B, T, _ = x.shape
         q, k, v = ops.multi_linear(x, (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight))
         q = q.view(B, T, self.num_heads, self.head_dim)
         k = k.view(B, T, self.num_kv_heads, self.head_dim)
         v = v.view(B, T, self.num_kv_heads, self.head_dim)
-        cos, sin = self.rotary_emb(x, position_ids, seq_len=T)
+        cos, sin = self.rotary_emb(x, position_ids, seq_len=T) if rotary is None else rotary(self.rotary_emb)
         q, k = apply_rotary_pos_emb(q, k, cos, sin)
         return q, k, v
 
     def forward(self, hidden_states: Tensor, attention_mask: Optional[Tensor] = None,
                 position_ids: Optional[Tensor] = None,
                 past_key_value: Optional[Tuple[Tensor, Tensor]] = None, use_cache: bool = False):
+        """``past_key_value`` is (keys, values) to be concatenated to, or one layer of a paged cache's step (``generation.LayerStep``), whose packed
+        tokens (1, N, hidden) know their positions."""
         B, T, _ = hidden_states.shape
+        if hasattr(past_key_value, "attend"):
+            q, k, v = self._qkv(hidden_states, None, past_key_value.rotary)
+            o = past_key_value.attend(q, k, v)
+            return self.o_proj(o.reshape(B, T, self.num_heads * self.head_dim)), None
         q, k, v = self._qkv(hidden_states, position_ids)
         if past_key_value is not None:
             k = torch.cat([past_key_value[0], k], dim=1)
@@ -145,6 +151,8 @@ class NativeSparseAttention(DenseAttention):
 
     def forward(self, hidden_states, attention_mask=None, position_ids=None,
                 past_key_value=None, use_cache: bool = False):
+        if hasattr(past_key_value, "attend"):
+            raise ValueError("the paged cache serves dense attention; sparse layers decode with use_cache=True")
         B, T, _ = hidden_states.shape
         q, k, v = self._qkv(hidden_states, position_ids)
         if past_key_value is not None:
@@ -218,9 +226,14 @@ class TransformerModel(CausalLMBase):
 
     def forward(self, input_ids: Tensor, attention_mask: Optional[Tensor] = None,
                 position_ids: Optional[Tensor] = None, past_key_values=None,
-                labels: Optional[Tensor] = None, use_cache: bool = False):
+                labels: Optional[Tensor] = None, use_cache: bool = False, return_hidden: bool = False):
+        """``past_key_values`` may be a step of a paged cache (``generation.CacheStep``): the tokens are then those of all its requests, packed as (1, N), and
+        nothing is returned in the cache's place.  ``return_hidden``: what the output head is applied to, in the place of the logits."""
         B, T = input_ids.shape
-        past_len = 0 if past_key_values is None else past_key_values[0][0].shape[1]
+        paged = hasattr(past_key_values, "plan")
+        if paged and (use_cache or B != 1 or labels is not None):
+            raise ValueError("a paged step takes packed tokens (1, N), without labels and use_cache")
+        past_len = 0 if past_key_values is None or paged else past_key_values[0][0].shape[1]
         if position_ids is None and past_len > 0:    # from position 0 the rotary tables are sliced by length
             position_ids = torch.arange(past_len, past_len + T, device=input_ids.device)
         h = self.embed_tokens(input_ids)
@@ -235,6 +248,8 @@ class TransformerModel(CausalLMBase):
             else:
                 h = self.run_layer(layer, h, attention_mask, position_ids)
         h = self.norm(h)
+        if return_hidden:
+            return h, None, caches
         logits, loss = self.compute_loss(h, labels)
         return logits, loss, caches
 

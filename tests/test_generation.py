@@ -1,0 +1,194 @@
+"""Generation and scoring through the paged 8-bit cache: on the CPU in fp32, on a GPU in bf16."""
+import pytest
+import torch
+
+from nsa_optim_b200 import ops
+from nsa_optim_b200.config import ModelConfig
+from nsa_optim_b200.generation import PagedCache, generate, score
+from nsa_optim_b200.models.hybrid import HybridConfig, create_hybrid_model
+from nsa_optim_b200.models.transformer import create_model
+
+
+@pytest.fixture(params=["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def dev(request):
+    yield request.param
+    if request.param == "cuda":
+        ops.native_module().check_status()
+
+
+def small(dev, attention="dense", heads=4, kv=2, head_dim=64, layers=2, vocab=512):
+    torch.manual_seed(3)
+    config = ModelConfig(name="small", hidden_size=256, intermediate_size=512, num_hidden_layers=layers, num_attention_heads=heads, num_key_value_heads=kv,
+                         head_dim=head_dim, vocab_size=vocab, max_position_embeddings=256, attention_type=attention)
+    model = create_model(config)
+    for p in model.parameters():
+        if p.dim() == 2:
+            torch.nn.init.normal_(p, std=0.06)
+    return model.to(dev, torch.bfloat16 if dev == "cuda" else torch.float32).eval()
+
+
+def texts(lengths, vocab=512):
+    g = torch.Generator().manual_seed(7)
+    return [torch.randint(0, vocab, (n,), generator=g).tolist() for n in lengths]
+
+
+def whole(model, ids, dev):
+    """Logits of a text by the ordinary forward."""
+    with torch.no_grad():
+        return model(torch.tensor([ids], device=dev))[0][0].float()
+
+
+def off(got, want):
+    return float((got.float() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("head_dim,heads,kv", [(64, 4, 2), (128, 8, 1)])
+def test_steps_agree_with_the_whole_text(dev, head_dim, heads, kv):
+    """Prompts, pieces and single tokens of requests of different lengths against the forward over the whole text.  Codes are off by up to half a step, a
+    step at most 2/127 of the page's largest number, about 3.5 times a typical one: 0.03 / sqrt(3) = 1.6 % of a key or a value, twice that of an
+    attention output with its probabilities, which the residual stream dilutes; 0.1 leaves a factor of three."""
+    model = small(dev, heads=heads, kv=kv, head_dim=head_dim)
+    ids = texts([90, 33, 70])
+    cache = PagedCache(model, requests=4, tokens=400, page_size=16)
+    at = [0, 0, 0, 0]
+    for new in ([40, 33, 0, 0], [1, 0, 17, 0], [1, 0, 1, 0], [0, 0, 30, 0], [48, 0, 22, 0]):
+        packed = [t for b in range(3) for t in ids[b][at[b]:at[b] + new[b]]]
+        step = cache.step(new)
+        with torch.no_grad():
+            logits = model(torch.tensor([packed], device=dev), past_key_values=step)[0][0]
+        row = 0
+        for b in range(3):
+            if new[b]:
+                assert off(logits[row:row + new[b]], whole(model, ids[b], dev)[at[b]:at[b] + new[b]]) < 0.1
+            row += new[b]
+            at[b] += new[b]
+        assert cache.lengths.tolist() == at and int(step.plan.shortfall) == 0
+    used = sum(-(-n // 16) for n in at)
+    assert int(cache.free_count) == cache.free.numel() - used
+    cache.release([True, False, True, False])
+    assert cache.lengths.tolist() == [0, 33, 0, 0] and int(cache.free_count) == cache.free.numel() - 3
+
+
+def test_greedy_tokens_are_the_likeliest(dev):
+    model = small(dev)
+    prompts = texts([5, 40, 1])
+    out = generate(model, prompts, 12, top_k=3, alternatives=True)
+    assert [len(t) for t in out.tokens] == [12] * 3
+    for b, p in enumerate(prompts):
+        logp = torch.log_softmax(whole(model, p + out.tokens[b], dev), -1)
+        for i, tok in enumerate(out.tokens[b]):
+            row = logp[len(p) + i - 1]
+            alts = out.alternatives[b][i]
+            assert alts[0] == (tok, out.logprobs[b][i]) and alts[0][1] >= alts[1][1] >= alts[2][1]
+            spread = float(row.max() - row.mean())
+            assert row[tok] >= row.max() - 0.1 * spread and abs(row[tok] - out.logprobs[b][i]) < 0.1 * spread
+            assert abs(out.entropies[b][i] + float((row.exp() * row).sum())) < 0.1 * spread
+
+
+def test_requests_do_not_see_one_another(dev):
+    """The same tokens whether a request runs alone or beside others that end earlier."""
+    model = small(dev)
+    prompts = texts([21, 64, 7, 30])
+    together = generate(model, prompts, 20)
+    end = together.tokens[1][4]
+    cut = generate(model, prompts, 20, end_token=end)
+    for b, p in enumerate(prompts):
+        alone = generate(model, [p], 20)
+        same = [x == y for x, y in zip(alone.tokens[0], together.tokens[b])]
+        first = same.index(False) if False in same else 20
+        if first < 20:                                       # products of other shapes round differently: only a near tie may fall otherwise
+            assert abs(alone.logprobs[0][first] - together.logprobs[b][first]) < 0.05
+        stop = together.tokens[b].index(end) + 1 if end in together.tokens[b] else 20
+        if first >= stop:
+            assert cut.tokens[b][:1] == together.tokens[b][:1] and (end not in cut.tokens[b][:-1])
+    assert len(cut.tokens[1]) <= 5 and cut.tokens[1][-1] == end
+
+
+def test_a_cache_is_used_again(dev):
+    model = small(dev)
+    cache = PagedCache(model, requests=3, tokens=120, page_size=32)
+    prompts = texts([30, 25])
+    first = generate(model, prompts, 6, cache=cache)
+    assert cache.lengths.tolist() == [0, 0, 0] and int(cache.free_count) == cache.free.numel()
+    assert sorted(cache.free.tolist()) == list(range(cache.free.numel()))
+    again = generate(model, prompts, 6, cache=cache)
+    assert first.tokens == again.tokens and first.logprobs == again.logprobs
+
+
+def test_sampling(dev):
+    model = small(dev)
+    prompts = texts([9, 12])
+    g = torch.Generator(device=dev).manual_seed(1)
+    out = generate(model, prompts, 30, temperature=1.0, top_k=5, alternatives=True, generator=g)
+    picks = [[t for t, _ in alts].index(tok) for b in range(2) for tok, alts in zip(out.tokens[b], out.alternatives[b])]
+    assert len(set(picks)) > 1 and max(picks) < 5
+    for b in range(2):
+        for tok, lp, alts in zip(out.tokens[b], out.logprobs[b], out.alternatives[b]):
+            assert dict(alts)[tok] == lp
+
+
+@pytest.mark.parametrize("kind", ["dense", "nsa", "hybrid"])
+def test_scores(dev, kind):
+    if kind == "hybrid":
+        torch.manual_seed(0)
+        model = create_hybrid_model(HybridConfig(d_model=256, vocab_size=512, block_pattern="MDA", block_repeats=1, num_attention_heads=4,
+                                                 num_key_value_heads=2, deltanet_head_dim=128, deltanet_num_heads=2, intermediate_size=512))
+        model = model.to(dev, torch.bfloat16 if dev == "cuda" else torch.float32).eval()
+    else:
+        model = small(dev, attention=kind)
+    ids = torch.tensor(texts([70, 70]), device=dev)
+    ids[1, 50:] = 0
+    r = score(model, ids, top_k=3, pad_token=0, chunk=33)
+    logits = model(ids)[0].detach().float()[:, :-1]
+    logp = torch.log_softmax(logits, -1)
+    want = logp.gather(-1, ids[:, 1:, None])[..., 0].masked_fill(ids[:, 1:] == 0, 0.0)
+    # the logits of other chunks of rows are rounded the same: only the log probability's own error, 2^-20 of numbers below 2^5, and in bf16 a last bit of
+    # the logits where a product is cut otherwise
+    tol = 2.0 ** -15 if dev == "cpu" else 2.0 ** -4
+    assert r.logprob.shape == (2, 69) and (r.logprob - want).abs().max() < tol
+    assert (r.entropy + (logp.exp() * logp).sum(-1)).abs().max() < tol
+    assert r.top_index.shape == (2, 69, 3) and (r.top_logprob - logp.topk(3).values).abs().max() < tol
+
+
+def test_refusals(dev):
+    model = small(dev, layers=1)
+    for bad in ([], [[]], [[1], []]):
+        with pytest.raises(ValueError):
+            generate(model, bad, 3)
+    for kw in (dict(max_new_tokens=0), dict(max_new_tokens=2, temperature=-1.0), dict(max_new_tokens=2, top_k=0)):
+        with pytest.raises(ValueError):
+            generate(model, [[1]], **kw)
+    cache = PagedCache(model, requests=1, tokens=64)
+    with pytest.raises(ValueError):
+        generate(model, [[1], [2]], 2, cache=cache)
+    for new in ([1, 1], [-1]):
+        with pytest.raises(ValueError):
+            cache.step(new)
+    with pytest.raises(ValueError):
+        model(torch.zeros(2, 3, dtype=torch.long, device=dev), past_key_values=cache.step([6]))
+    with pytest.raises(ValueError):
+        model(torch.zeros(1, 3, dtype=torch.long, device=dev), past_key_values=cache.step([3]), use_cache=True)
+    with pytest.raises(ValueError):
+        PagedCache(small(dev, attention="nsa", layers=1), requests=1, tokens=64)
+    with pytest.raises(ValueError):
+        score(model, torch.zeros(4, dtype=torch.long, device=dev))
+
+
+@pytest.mark.gpu
+def test_a_step_is_native(native):
+    """No part of a step runs on the PyTorch implementation, and nothing waits for the device."""
+    model = small("cuda")
+    cache = PagedCache(model, requests=2, tokens=200)
+    ids = torch.tensor([texts([50])[0]], device="cuda")
+    rows = torch.tensor([0], device="cuda")
+    for new in ([30, 20], [1, 1]):
+        native.fallback_counts(reset=True)
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            with torch.no_grad():
+                h = model(ids[:, :sum(new)], past_key_values=cache.step(new), return_hidden=True)[0]
+                ops.token_logprobs(ops.linear(h[0, rows], model.output_weight()), rows, 4)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+        assert native.fallback_counts() == {}
