@@ -3,17 +3,17 @@
 // o = sum_j 2^(x_j - M) v_j / sum_j 2^(x_j - M), x_j = log2(e) scale q k_j, in one pass with a running M.  Rows are (query token, head of the KV head's
 // group) pairs, 16 to a warp's matrix product (m16n8k16 on f16), so a group shares what it reads.  With few rows the bytes of the codes bound it;
 // every other choice serves that:
-//  * Work is counted in units of 64 keys, over all requests, KV heads and row tiles, and dealt out evenly to workers (a warp with 16 rows, more
-//    warps on the same keys where a request has more rows): ragged requests cost no more than even ones.  A worker's range may end inside a request;
-//    such parts meet in shared memory at the CTA's end, and across CTAs in cache_attn_join_kernel.
+//  * Work is counted in units of 64 keys, over all requests, KV heads and row tiles, and dealt out evenly to workers, a warp each: ragged requests cost
+//    no more than even ones.  A worker's range may end inside a request; such parts meet in shared memory at the CTA's end, and across CTAs in
+//    cache_attn_join_kernel.
 //  * Each worker has its own ring of key and value tiles that asynchronous copies fill two tiles ahead: 130 KB in flight per SM, no registers, and no
 //    synchronisation between workers.
 //  * The cache's orders are those of the product's operands.  Of a unit, lane 4c+r of a warp scores token 2j + c%2 of sub-block c/2 in tile j and holds
 //    the probabilities of sub-block r's tokens 2j, 2j+1, so its value operand is 16 neighbouring bytes.
 //  * A code u becomes an f16 operand by a byte permutation alone: the bits 0x00uu are the (subnormal) number 2^-24 u.  The offset of 128 comes out
 //    of sums: 128 sum(q) of a row's scores, and 128 sum(p) of its outputs, which one more product per step leaves in the accumulators' format and
-//    which is taken off every fourth unit, before it outgrows them.  (With a subtraction per pair of codes, 256 of 1170 instructions a unit, 64
-//    contexts of up to 8192 tokens took XX us.)
+//    which is taken off every fourth unit, before it outgrows them.  (With a subtraction per pair of codes, 256 of 1170 instructions a unit, drafts for
+//    32 contexts of up to 12000 tokens took 268 us, then 240.)
 //  * Codes and their products are exact, and so is a query row scaled by a power of two to 2^13 .. 2^14 (bf16's 8 bits; what is 2^-28 of the row's
 //    largest value rounds).  Probabilities are rounded to 11 bits, relative to the row's largest product of probability and value scale: the value
 //    scale's exponent is added to x, and taken out again of the sum.  Sums are fp32.
@@ -55,14 +55,13 @@ struct alignas(16) Join {
   long long end, each;  // the unit at which it ends, units of a worker
 };
 
-template <int D, int MT>
+template <int D>
 struct Shape {
-  static constexpr int kRows = 16 * MT, kGroups = kWarps / MT;         // rows and workers of a CTA
   static constexpr int kSub = 16 * D, kPitch = kSub + 32;              // a sub-block of 16 tokens; the pitch spreads four of them over the banks
   static constexpr int kSlot = 4 * kPitch;                             // a unit's keys or values
-  static constexpr int kSlots = 24 * (128 / D) / kGroups;              // of a worker
+  static constexpr int kSlots = 3 * (128 / D);                         // of a worker
   static constexpr int kRing = kSlots * kSlot;
-  static_assert(kRing >= kRows * D * 4, "a worker's sums go where its ring was");
+  static_assert(kRing >= 16 * D * 4, "a worker's sums go where its ring was");
 };
 
 __device__ __forceinline__ int token_of(const AttnParams& p, int row) { return static_cast<int>(static_cast<unsigned>(row) * p.per_g >> 32); }
@@ -84,14 +83,14 @@ struct Request {
   __device__ __forceinline__ int units(int window) const { return n > 0 ? max(((cap + 63) >> 6) - unit0(window), 1) : 0; }
 };
 
-template <int D, int MT>
+template <int D, int R>
 struct Smem {
-  using S = Shape<D, MT>;
-  alignas(128) uint8_t ring[S::kGroups][S::kRing];
-  float2 scale[S::kGroups][S::kSlots][4];
-  uint64_t full[S::kGroups][S::kSlots], empty[S::kGroups][S::kSlots];
-  float2 ml[S::kGroups][2][S::kRows];
-  Left left[S::kGroups];
+  using S = Shape<D>;
+  alignas(128) uint8_t ring[kWarps][S::kRing];
+  float2 scale[kWarps][S::kSlots][4];
+  uint64_t full[kWarps][S::kSlots];
+  float2 ml[kWarps][2][R];
+  Left left[kWarps];
   long long before[kMaxRequests + 1];                                  // units of the requests before b
   Request request[kMaxRequests];
   long long warps[kWarps];
@@ -230,16 +229,126 @@ __device__ __forceinline__ float log2_of_scale(float s) {
   return e > 60 ? CUDART_NAN_F : static_cast<float>(e);
 }
 
-// A warp's 16 rows: queries as f16 operands, running maximum, sum, output
+// Queries of one row, columns 16 r .. 16 r + 15 of each 64 for lane r of a quad.  Asked for first, taken up when the copies are under way: behind them
+// they would wait for 30 MB (7000 cycles).
 template <int D>
-struct Rows {
-  uint32_t q[D / 16][4];
-  float factor[2];      // of lane rows r and r + 8: takes a product of f16 queries and code numbers to 2^-24 x / key scale
-  float off[2];         // what the codes' offset adds to such a product
-  int pos[2];           // their positions; -1: no row
+struct Query {
+  uint4 v[D / 64][2];
+  __device__ __forceinline__ void ask(const AttnParams& p, const Piece& it, int row) {
+    const int t = token_of(p, row);
+    const bf16* src = p.q + static_cast<long>(it.q0 + t) * p.ldq + static_cast<long>(it.h * p.G + row - t * p.G) * D + (threadIdx.x & 3) * 16;
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) v[h][k] = t < it.n ? *reinterpret_cast<const uint4*>(src + h * 64 + k * 8) : make_uint4(0, 0, 0, 0);
+  }
+  // As f16 numbers, scaled; factor takes a product with code numbers to 2^-24 x / key scale, off is what the codes' offset adds to such a product
+  __device__ __forceinline__ void take(float softmax_scale, uint32_t (&q)[D / 16][2], float& factor, float& off) const {
+    unsigned top = 0;
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t w[4] = {v[h][k].x, v[h][k].y, v[h][k].z, v[h][k].w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) top = max(top, max(w[y] & 0x7fffu, (w[y] >> 16) & 0x7fffu));
+      }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = static_cast<int>(top >> 7);                          // the largest magnitude is 2^(e - 127) at least
+    const int up = min(140 - e, 126);
+    const float f = softmax_scale < 0.f ? -__int_as_float((up + 127) << 23) : __int_as_float((up + 127) << 23);
+    factor = e == 255 ? CUDART_NAN_F : __int_as_float((127 - up) << 23) * fabsf(softmax_scale);
+    float sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t w[4] = {v[h][k].x, v[h][k].y, v[h][k].z, v[h][k].w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {                                  // columns 16 r + 8 k + 2 y, + 1 of this half
+          const float a = __int_as_float(w[y] << 16) * f, b = __int_as_float(w[y] & 0xffff0000u) * f;
+          sum += a + b;
+          q[h * 4 + k * 2 + (y >> 1)][y & 1] = pack_half(a, b);
+        }
+      }
+    off = quad_sum(sum) * 0x1p-17f;
+  }
+};
+
+// Scores s of two rows and some keys of a lane become probabilities.  get(row, n) is the reference to its n-th score, key(n) that one's token in the
+// lane's sub-block, N of them; reduce() the maximum over the lanes that share the rows, rescale(f) multiplies their outputs.
+struct Running {
+  float factor[2], off[2];   // of the lane's two rows
+  int pos[2];                // their positions; -1: no row
   float m[2], l[2];
-  float o[D / 8][4];    // with 128 times the sum of probabilities still in it, whose negative `off_o` is
-  float off_o[4];
+};
+template <int N, class Get, class Key, class Reduce, class Rescale>
+__device__ __forceinline__ void references(Running& w, Get get, Key key, Reduce reduce, Rescale rescale, float2 scale, bool masked, int key0, int window,
+                                           float (&a)[2], float (&b)[2], float& out) {
+  const bool there = scale.x != 0.f;                                   // else a sub-block without a page
+  const float ev = there ? log2_of_scale(scale.y) : 0.f, sk = there ? scale.x * 0x1p24f : 0.f;
+  float c[2], top[2], ref[2];                                          // x = a s + c, a > 0
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    a[i] = w.factor[i] * sk;
+    a[i] = a[i] == 0.f ? 0x1p-126f : a[i];
+    c[i] = fmaf(-w.off[i], a[i], ev);
+    top[i] = -CUDART_INF_F;
+  }
+  if (masked) {                                                        // some key of the unit is not seen by some row: such scores become -inf
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int to = there ? w.pos[i] - key0 : -1, from = window > 0 ? w.pos[i] - window - key0 : -1;      // from < key <= to
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (key(n) > to || key(n) <= from) get(i, n) = -CUDART_INF_F;
+      if (to < 0 || from >= 15 || from >= to) {                        // a row that sees nothing of a page does not see that its scale is NaN
+        a[i] = 1.f;
+        c[i] = 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    top[0] = fmaxf(top[0], get(0, n));
+    top[1] = fmaxf(top[1], get(1, n));
+  }
+  bool moved = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float m = fmaxf(w.m[i], reduce(fmaf(top[i], a[i], c[i])));
+    moved |= m != w.m[i];
+    ref[i] = m == -CUDART_INF_F ? 0.f : m;
+    top[i] = m;
+    b[i] = c[i] - ref[i];
+  }
+  if (__any_sync(0xffffffffu, moved)) {
+    const float2 f = make_float2(ex2(w.m[0] - ref[0]), ex2(w.m[1] - ref[1]));
+    w.m[0] = top[0];
+    w.m[1] = top[1];
+    w.l[0] *= f.x;
+    w.l[1] *= f.y;
+    rescale(f);
+  }
+  out = ex2(-ev);
+}
+__device__ __forceinline__ void add_sum(float& l, float t, float out) { l += t == 0.f ? 0.f : t * out; }
+
+// A warp's rows: queries as f16 operands, running maximum and sum, outputs.  The outputs have 128 times the sum of probabilities still in them, whose
+// negative is off_o.
+template <int D, int R>
+struct Rows;
+
+// 16 rows: scores S = Q K^T, lane 4c + r has rows c and c + 8, keys of sub-block r; outputs P V, the same rows, columns 8 d + 2 r, + 1
+template <int D>
+struct Rows<D, 16> : Running {
+  using S = Shape<D>;
+  Query<D> raw[2];
+  uint32_t q[D / 16][4], pr[8][2];
+  float o[D / 8][4], off_o[4];
+  static __device__ __forceinline__ int sub_block() { return threadIdx.x & 3; }          // of a lane's keys
+  static __device__ __forceinline__ int row(int i) { return (threadIdx.x & 31) / 4 + 8 * i; }
 
   __device__ __forceinline__ void clear() {
     m[0] = m[1] = -CUDART_INF_F;
@@ -257,189 +366,247 @@ struct Rows {
     }
     off_o[0] = off_o[1] = off_o[2] = off_o[3] = 0.f;
   }
-
-  // Row r of the item is query token r / G, head r % G of the group.  Asked for first, taken up when the copies are under way: behind them they
-  // would wait for 30 MB (7000 cycles).
-  struct Raw {
-    uint4 v[2][D / 64][2];
-  };
-  __device__ __forceinline__ void ask(Raw& raw, const AttnParams& p, const Piece& it, int row0) {
-    const int lane = threadIdx.x & 31, r = lane & 3;
+  __device__ __forceinline__ void ask(const AttnParams& p, const Piece& it, int row0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) raw[i].ask(p, it, row0 + row(i));
+  }
+  __device__ __forceinline__ void take(float softmax_scale) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int row = row0 + (lane >> 2) + 8 * i, t = token_of(p, row);
-      const bool there = t < it.n;
-      pos[i] = there ? it.past + t : -1;
-      const bf16* src = p.q + static_cast<long>(it.q0 + t) * p.ldq + static_cast<long>(it.h * p.G + row - t * p.G) * D + r * 16;
+      uint32_t half[D / 16][2];
+      raw[i].take(softmax_scale, half, factor[i], off[i]);
 #pragma unroll
-      for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) raw.v[i][h][k] = there ? *reinterpret_cast<const uint4*>(src + h * 64 + k * 8) : make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < D / 16; ++k) {
+        q[k][i] = half[k][0];
+        q[k][i + 2] = half[k][1];
+      }
     }
   }
-  __device__ __forceinline__ void take(const Raw& raw, float softmax_scale) {
+  __device__ __forceinline__ void keys(const uint8_t* tile, float2 scale, bool masked, int key0, int window) {
+    const int lane = threadIdx.x & 31, c = lane >> 2, r = lane & 3;
+    const uint8_t* base = tile + (c >> 1) * S::kPitch + (c & 1) * 64 + r * 16;
+    float s[8][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      unsigned top = 0;
+    for (int j = 0; j < 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
-      for (int h = 0; h < D / 64; ++h)
+    for (int g = 0; g < 8; g += 4)                                     // four tiles at a time: their products do not wait for one another
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t w[4] = {raw.v[i][h][k].x, raw.v[i][h][k].y, raw.v[i][h][k].z, raw.v[i][h][k].w};
+      for (int h = 0; h < D / 64; ++h) {
+        uint32_t words[4][4];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) top = max(top, max(w[y] & 0x7fffu, (w[y] >> 16) & 0x7fffu));
-        }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = static_cast<int>(top >> 7);                        // the largest magnitude is 2^(e - 127) at least
-      const int up = min(140 - e, 126);
-      const float f = softmax_scale < 0.f ? -__int_as_float((up + 127) << 23) : __int_as_float((up + 127) << 23);
-      factor[i] = e == 255 ? CUDART_NAN_F : __int_as_float((127 - up) << 23) * fabsf(softmax_scale);
-      float sum = 0.f;
+        for (int j = 0; j < 4; ++j) load4(words[j], base + ((g + j) * (D / 64) + h) * 128);
 #pragma unroll
-      for (int h = 0; h < D / 64; ++h)
+        for (int y = 0; y < 4; ++y)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t w[4] = {raw.v[i][h][k].x, raw.v[i][h][k].y, raw.v[i][h][k].z, raw.v[i][h][k].w};
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {                                // columns 16 r + 8 k + 2 y, + 1 of this half
-            const float a = __int_as_float(w[y] << 16) * f, b = __int_as_float(w[y] & 0xffff0000u) * f;
-            sum += a + b;
-            q[h * 4 + k * 2 + (y >> 1)][i + 2 * (y & 1)] = pack_half(a, b);
+          for (int j = 0; j < 4; ++j) {
+            uint32_t b0, b1;
+            decode(words[j][y], b0, b1);
+            mma(s[g + j], q[h * 4 + y], b0, b1);
           }
-        }
-      off[i] = quad_sum(sum) * 0x1p-17f;
-    }
-  }
-};
-
-// Scores of one unit (codes' products): s[j] are tile j's
-template <int D, class S>
-__device__ __forceinline__ void scores(const Rows<D>& w, const uint8_t* keys, float (&s)[8][4]) {
-  const int lane = threadIdx.x & 31, c = lane >> 2, r = lane & 3;
-  const uint8_t* base = keys + (c >> 1) * S::kPitch + (c & 1) * 64 + r * 16;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-#pragma unroll
-  for (int g = 0; g < 8; g += 4)                                       // four tiles at a time: their products do not wait for one another
-#pragma unroll
-    for (int h = 0; h < D / 64; ++h) {
-      uint32_t words[4][4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) load4(words[j], base + ((g + j) * (D / 64) + h) * 128);
-#pragma unroll
-      for (int y = 0; y < 4; ++y)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t b0, b1;
-          decode(words[j][y], b0, b1);
-          mma(s[g + j], w.q[h * 4 + y], b0, b1);
-        }
-    }
-}
-
-// Scores to probabilities, in f16 pairs, with the running maximum and sum.  masked: some key of the unit is not seen by some row; such scores become
-// -inf, before x = a s + c with a > 0.
-template <int D>
-__device__ __forceinline__ void softmax(Rows<D>& w, float (&s)[8][4], uint32_t (&pr)[8][2], float2 scale, bool masked, int key0, int window) {
-  const bool there = scale.x != 0.f;                                   // else a sub-block without a page
-  const float ev = there ? log2_of_scale(scale.y) : 0.f, sk = there ? scale.x * 0x1p24f : 0.f;
-  float a[2], c[2], top[2], ref[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    a[i] = w.factor[i] * sk;
-    a[i] = a[i] == 0.f ? 0x1p-126f : a[i];
-    c[i] = fmaf(-w.off[i], a[i], ev);
-    top[i] = -CUDART_INF_F;
-  }
-  if (masked) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      // keys 2j + e of the lane's sub-block with from < 2j + e <= to
-      const int to = there ? w.pos[i] - key0 : -1, from = window > 0 ? w.pos[i] - window - key0 : -1;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (2 * j + e > to || 2 * j + e <= from) s[j][2 * i + e] = -CUDART_INF_F;
-      if (to < 0 || from >= 15 || from >= to) {                        // a row that sees nothing of a page does not see that its scale is NaN
-        a[i] = 1.f;
-        c[i] = 0.f;
       }
-    }
-  }
+    float a[2], b[2], out;
+    references<16>(
+        *this, [&](int i, int n) -> float& { return s[n >> 1][2 * i + (n & 1)]; }, [](int n) { return n; }, [](float x) { return quad_max(x); },
+        [&](float2 f) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+          for (int i = 0; i < 4; ++i) off_o[i] *= i < 2 ? f.x : f.y;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top[i >> 1] = fmaxf(top[i >> 1], s[j][i]);
-  bool moved = false;
+          for (int d = 0; d < D / 8; ++d) {
+            float2* x = reinterpret_cast<float2*>(o[d]);
+            x[0] = mul2(x[0], make_float2(f.x, f.x));
+            x[1] = mul2(x[1], make_float2(f.y, f.y));
+          }
+        },
+        scale, masked, key0, window, a, b, out);
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float m = fmaxf(w.m[i], quad_max(fmaf(top[i], a[i], c[i])));
-    moved |= m != w.m[i];
-    ref[i] = m == -CUDART_INF_F ? 0.f : m;
-    top[i] = m;
-  }
-  if (__any_sync(0xffffffffu, moved)) {
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float f = ex2(w.m[i] - ref[i]);
-      w.m[i] = top[i];
-      w.l[i] *= f;
-      w.off_o[2 * i] *= f;
-      w.off_o[2 * i + 1] *= f;
-#pragma unroll
-      for (int d = 0; d < D / 8; ++d) {
-        float2* o = reinterpret_cast<float2*>(w.o[d]);
-        o[i] = mul2(o[i], make_float2(f, f));
+      for (int i = 0; i < 2; ++i) {
+        const float2 x = fma2(make_float2(s[j][2 * i], s[j][2 * i + 1]), make_float2(a[i], a[i]), make_float2(b[i], b[i]));
+        const float2 e = make_float2(ex2(x.x), ex2(x.y));
+        sum[i] = add2(sum[i], e);
+        pr[j][i] = pack_half(e.x, e.y);
       }
-    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) add_sum(l[i], sum[i].x + sum[i].y, out);
   }
-  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float b = c[i] - ref[i];
-      const float2 x = fma2(make_float2(s[j][2 * i], s[j][2 * i + 1]), make_float2(a[i], a[i]), make_float2(b, b));
-      const float2 e = make_float2(ex2(x.x), ex2(x.y));
-      sum[i] = add2(sum[i], e);
-      pr[j][i] = pack_half(e.x, e.y);
-    }
-  const float out = ex2(-ev);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float t = sum[i].x + sum[i].y;
-    w.l[i] += t == 0.f ? 0.f : t * out;
-  }
-}
-
-template <int D, class S>
-__device__ __forceinline__ void accumulate(Rows<D>& w, const uint8_t* values, const uint32_t (&pr)[8][2]) {
-  const int lane = threadIdx.x & 31;
-  const uint8_t* base = values + (lane & 3) * S::kPitch + (lane >> 2) * 16;
-#pragma unroll
-  for (int y = 0; y < 4; ++y) {
-    const uint32_t a[4] = {pr[2 * y][0], pr[2 * y][1], pr[2 * y + 1][0], pr[2 * y + 1][1]};
-    mma(w.off_o, a, kMinus128, kMinus128);
-  }
-#pragma unroll
-  for (int g = 0; g < D / 8; g += 4) {
-    uint32_t words[4][4];
-#pragma unroll
-    for (int d = 0; d < 4; ++d) load4(words[d], base + (g + d) * 128);
+  __device__ __forceinline__ void values(const uint8_t* tile) {
+    const int lane = threadIdx.x & 31;
+    const uint8_t* base = tile + (lane & 3) * S::kPitch + (lane >> 2) * 16;
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       const uint32_t a[4] = {pr[2 * y][0], pr[2 * y][1], pr[2 * y + 1][0], pr[2 * y + 1][1]};
+      mma(off_o, a, kMinus128, kMinus128);
+    }
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        uint32_t b0, b1;
-        decode(words[d][y], b0, b1);
-        mma(w.o[g + d], a, b0, b1);
+    for (int g = 0; g < D / 8; g += 4) {
+      uint32_t words[4][4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) load4(words[d], base + (g + d) * 128);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t a[4] = {pr[2 * y][0], pr[2 * y][1], pr[2 * y + 1][0], pr[2 * y + 1][1]};
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          uint32_t b0, b1;
+          decode(words[d][y], b0, b1);
+          mma(o[g + d], a, b0, b1);
+        }
       }
     }
   }
-}
+  __device__ __forceinline__ void sums() {
+    settle();
+    l[0] = quad_sum(l[0]);
+    l[1] = quad_sum(l[1]);
+  }
+  __device__ __forceinline__ bool writes_sums() const { return (threadIdx.x & 3) == 0; }
+  // Row i's outputs times f: as bf16, and as they are
+  __device__ __forceinline__ void store(bf16* out, int i, float f) const {
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d)
+      *reinterpret_cast<__nv_bfloat162*>(out + d * 8 + (threadIdx.x & 3) * 2) = __floats2bfloat162_rn(o[d][2 * i] * f, o[d][2 * i + 1] * f);
+  }
+  __device__ __forceinline__ void store(float* out, int i) const {
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(out + d * 8 + (threadIdx.x & 3) * 2) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+  }
+};
+
+// 8 rows: scores transposed, S^T = K Q^T, lane 4c + r has rows 2r and 2r + 1, keys of sub-block c / 2; outputs O^T = V^T P^T, the same rows, columns
+// 16 d + c, + 8.  Half the products and exponentials for the same codes; the probabilities change lanes once (movmatrix).
+template <int D>
+struct Rows<D, 8> : Running {
+  using S = Shape<D>;
+  Query<D> raw;
+  uint32_t q[D / 16][2], pr[4][2];
+  float o[D / 16][4], off_o[4];
+  static __device__ __forceinline__ int sub_block() { return (threadIdx.x & 31) >> 3; }
+  static __device__ __forceinline__ int row(int i) { return (threadIdx.x & 3) * 2 + i; }
+
+  __device__ __forceinline__ void clear() {
+    m[0] = m[1] = -CUDART_INF_F;
+    l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    off_o[0] = off_o[1] = off_o[2] = off_o[3] = 0.f;
+  }
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      float2* x = reinterpret_cast<float2*>(o[i]);
+      x[0] = add2(x[0], make_float2(off_o[0], off_o[1]));
+      x[1] = add2(x[1], make_float2(off_o[2], off_o[3]));
+    }
+    off_o[0] = off_o[1] = off_o[2] = off_o[3] = 0.f;
+  }
+  __device__ __forceinline__ void ask(const AttnParams& p, const Piece& it, int row0) { raw.ask(p, it, row0 + (threadIdx.x & 31) / 4); }
+  __device__ __forceinline__ void take(float softmax_scale) {
+    float f, c;
+    raw.take(softmax_scale, q, f, c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      factor[i] = __shfl_sync(0xffffffffu, f, row(i) * 4);
+      off[i] = __shfl_sync(0xffffffffu, c, row(i) * 4);
+    }
+  }
+  static __device__ __forceinline__ float over_keys(float x, bool sum) {
+#pragma unroll
+    for (int d = 4; d < 32; d *= 2) {
+      const float y = __shfl_xor_sync(0xffffffffu, x, d);
+      x = sum ? x + y : fmaxf(x, y);
+    }
+    return x;
+  }
+  __device__ __forceinline__ void keys(const uint8_t* tile, float2 scale, bool masked, int key0, int window) {
+    const int lane = threadIdx.x & 31, c = lane >> 2, r = lane & 3;
+    const uint8_t* base = tile + (c >> 1) * S::kPitch + (c & 1) * 64 + r * 16;
+    float s[4][4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) s[y][0] = s[y][1] = s[y][2] = s[y][3] = 0.f;
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) {
+      uint32_t words[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) load4(words[j], base + (j * (D / 64) + h) * 128);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          uint32_t a[4];
+          decode(words[2 * y][k], a[0], a[2]);
+          decode(words[2 * y + 1][k], a[1], a[3]);
+          mma(s[y], a, q[h * 4 + k][0], q[h * 4 + k][1]);
+        }
+    }
+    float a[2], b[2], out;
+    // score n of row i: token 2n + c % 2
+    references<8>(
+        *this, [&](int i, int n) -> float& { return s[n >> 1][2 * (n & 1) + i]; }, [&](int n) { return 2 * n + (c & 1); },
+        [](float x) { return over_keys(x, false); },
+        [&](float2 f) {
+          float2* t = reinterpret_cast<float2*>(off_o);
+          t[0] = mul2(t[0], f);
+          t[1] = mul2(t[1], f);
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            float2* x = reinterpret_cast<float2*>(o[d]);
+            x[0] = mul2(x[0], f);
+            x[1] = mul2(x[1], f);
+          }
+        },
+        scale, masked, key0, window, a, b, out);
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float2 x = fma2(make_float2(s[y][2 * t], s[y][2 * t + 1]), make_float2(a[0], a[1]), make_float2(b[0], b[1]));
+        const float2 e = make_float2(ex2(x.x), ex2(x.y));
+        sum = add2(sum, e);
+        asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pr[y][t]) : "r"(pack_half(e.x, e.y)));
+      }
+    add_sum(l[0], sum.x, out);
+    add_sum(l[1], sum.y, out);
+  }
+  __device__ __forceinline__ void values(const uint8_t* tile) {
+    const int lane = threadIdx.x & 31;
+    const uint8_t* base = tile + (lane & 3) * S::kPitch + (lane >> 2) * 16;
+    const uint32_t minus[4] = {kMinus128, kMinus128, kMinus128, kMinus128};
+#pragma unroll
+    for (int y = 0; y < 4; ++y) mma(off_o, minus, pr[y][0], pr[y][1]);
+#pragma unroll
+    for (int g = 0; g < D / 16; g += 4) {
+      uint32_t words[8][4];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) load4(words[d], base + (2 * g + d) * 128);
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          uint32_t a[4];
+          decode(words[2 * d][y], a[0], a[2]);
+          decode(words[2 * d + 1][y], a[1], a[3]);
+          mma(o[g + d], a, pr[y][0], pr[y][1]);
+        }
+    }
+  }
+  __device__ __forceinline__ void sums() {
+    settle();
+    l[0] = over_keys(l[0], true);
+    l[1] = over_keys(l[1], true);
+  }
+  __device__ __forceinline__ bool writes_sums() const { return (threadIdx.x & 31) < 4; }
+  __device__ __forceinline__ void store(bf16* out, int i, float f) const {
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d) out[d * 8 + (threadIdx.x & 31) / 4] = __float2bfloat16(o[d / 2][i + 2 * (d & 1)] * f);
+  }
+  __device__ __forceinline__ void store(float* out, int i) const {
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d) out[d * 8 + (threadIdx.x & 31) / 4] = o[d / 2][i + 2 * (d & 1)];
+  }
+};
 
 // Where row r of an item goes; nullptr: there is no such row
 __device__ __forceinline__ bf16* row_of(const AttnParams& p, int n, int q0, int h, int row, int D) {
@@ -449,20 +616,17 @@ __device__ __forceinline__ bf16* row_of(const AttnParams& p, int n, int q0, int 
 // What takes sums of probabilities and code numbers to the output
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 0x1p24f / l; }
 
-template <int D, int MT>
+template <int D, int R>
 __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_constant__ AttnParams p) {
-  using S = Shape<D, MT>;
+  using S = Shape<D>;
   extern __shared__ __align__(128) uint8_t raw_smem[];
-  Smem<D, MT>& sm = *reinterpret_cast<Smem<D, MT>*>(raw_smem);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tc5::warp_index(), grp = warp / MT, mt = warp % MT, B = p.s.B;
+  Smem<D, R>& sm = *reinterpret_cast<Smem<D, R>*>(raw_smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tc5::warp_index(), B = p.s.B;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- the units of all requests
   if (tid == 0) sm.abort_flag = 0;
-  for (int i = tid; i < S::kGroups * S::kSlots; i += kThreads) {
-    tc5::mbar_init(&sm.full[0][0] + i, 32);
-    tc5::mbar_init(&sm.empty[0][0] + i, MT);
-  }
+  for (int i = tid; i < kWarps * S::kSlots; i += kThreads) tc5::mbar_init(&sm.full[0][0] + i, 32);
   tc5::fence_barrier_init();
   asm volatile("griddepcontrol.wait;" ::: "memory");                   // until here the kernel may run beside the one before it
   long long total = 0;
@@ -472,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
     if (b < B) {
       const Request r = request_of(p, b);
       sm.request[b] = r;
-      x = static_cast<long long>(r.units(p.window)) * p.c.H * ((r.n * p.G + S::kRows - 1) / S::kRows);
+      x = static_cast<long long>(r.units(p.window)) * p.c.H * ((r.n * p.G + R - 1) / R);
     }
     const long long mine = x;
     for (int d = 1; d < 32; d <<= 1) {
@@ -493,14 +657,14 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
   __syncthreads();
 
   // ---- this worker's range
-  const long long workers = static_cast<long long>(gridDim.x) * S::kGroups, each = max((total + workers - 1) / workers, 1ll);
-  const long long begin = min((static_cast<long long>(blockIdx.x) * S::kGroups + grp) * each, total);
-  Cursor<S::kRows> use, get;
+  const long long workers = static_cast<long long>(gridDim.x) * kWarps, each = max((total + workers - 1) / workers, 1ll);
+  const long long begin = min((static_cast<long long>(blockIdx.x) * kWarps + warp) * each, total);
+  Cursor<R> use, get;
   use.init(p, sm.before, sm.request, begin, min(begin + each, total));
   get = use;
 
   // ---- the producer's side: tile t of the range is the keys (even) or values (odd) of its unit t / 2
-  uint8_t* ring = sm.ring[grp];
+  uint8_t* ring = sm.ring[warp];
   int get_unit = 0, get_stop = 0;                                      // of the piece that `get` is in
   struct Where {
     int page, blk, head;
@@ -525,19 +689,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
     ++get_unit;
   };
   int put = 0;                                                         // the slot of the next tile
-  uint32_t put_round = 0;
   bool values = false;
-  auto issue = [&](bool& ok) {                                         // the next tile, if there is one
+  auto issue = [&]() {                                         // the next tile, if there is one
     if (!values) look();
     if (!now.have) return;
     const int slot = put;
-    if (MT > 1 && put_round > 0)
-      ok = ok && tc5::mbar_wait_warp(&sm.empty[grp][slot], (put_round - 1) & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_EMPTY);
-    if (!ok) return;
-    if (++put == S::kSlots) {
-      put = 0;
-      ++put_round;
-    }
+    if (++put == S::kSlots) put = 0;
     // 16 bytes at a time by all lanes: a 2 KB bulk copy per sub-block took its lane 110 cycles, 520 a tile, in the way of the products
     const bool there = now.page >= 0 && now.page < p.c.pages;
     const long ph = static_cast<long>(there ? now.page : 0) * p.c.H + now.head;
@@ -553,34 +710,31 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + sub * S::kPitch + k * 512), "l"(src + k * 512) : "memory");
     }
     if (!values && lane < 4)                                           // zeros where there is no page
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(tc5::smem_u32(&sm.scale[grp][slot][lane])), "l"(p.c.scale + ph * 2),
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(tc5::smem_u32(&sm.scale[warp][slot][lane])), "l"(p.c.scale + ph * 2),
                    "r"(there ? 8 : 0)
                    : "memory");
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc5::smem_u32(&sm.full[grp][slot])) : "memory");
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc5::smem_u32(&sm.full[warp][slot])) : "memory");
     values = !values;
   };
   bool ok = true;
 
   // ---- the consumer's side
-  Rows<D> w;
-  typename Rows<D>::Raw raw;
+  Rows<D, R> w;
   int slot = 0;                                                        // of the next tile, and how often the ring has gone round
   uint32_t round = 0;
   Left left{};
   left.some = use.at < use.end;
   Piece it{};
   bool held = false;                                                   // whether there is a piece whose sums are in w
-  const int r = lane >> 2, col = (lane & 3) * 2;
-  uint32_t pr[8][2];
-  int u2 = 0, u2_end = 0, p0 = -1, p1 = -1, ahead = S::kSlots + 1, row0 = 0;
+  int u2 = 0, u2_end = 0, p0 = -1, p1 = -1, ahead = S::kSlots + 1;
   bool full = false, start = true, fresh = false;
   // One copy of the code at each place: 99 KB of instructions, with two, cost 10000 cycles a call in first fetches.  A turn issues a tile and takes one
   // up; keys and values of a unit take turns.  The first turn asks for queries, the next only issue (two of them only look up pages), so that a
   // tile is issued when the one that was in its place has been taken up.
 #pragma unroll 1
   for (;;) {
-    if (mt == 0 && !start) {
-      issue(ok);
+    if (!start) {
+      issue();
       if (ahead > 0) {
         --ahead;
         continue;
@@ -589,64 +743,53 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
     while (u2 >= u2_end) {
       const long long piece_end = use.at;
       const bool more = use.next_piece(p, sm.before, sm.request);
-      if (more) w.ask(raw, p, use.p, use.p.row0 + mt * 16);            // arrives while the sums before are stored
+      if (more) w.ask(p, use.p, use.p.row0);                           // arrives while the sums before are stored
       if (held) {
-        w.settle();
-        w.l[0] = quad_sum(w.l[0]);
-        w.l[1] = quad_sum(w.l[1]);
-        if (!it.began && !it.open) {                                     // the whole item: its rows are done
+        w.sums();
+        if (!it.began && !it.open) {                                   // the whole item: its rows are done
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            bf16* out = row_of(p, it.n, it.q0, it.h, it.row0 + mt * 16 + r + 8 * i, D);
-            if (out) {
-              const float f = inverse(w.l[i]);
-#pragma unroll
-              for (int d = 0; d < D / 8; ++d)
-                *reinterpret_cast<__nv_bfloat162*>(out + d * 8 + col) = __floats2bfloat162_rn(w.o[d][2 * i] * f, w.o[d][2 * i + 1] * f);
-            }
+            bf16* out = row_of(p, it.n, it.q0, it.h, it.row0 + w.row(i), D);
+            if (out) w.store(out, i, inverse(w.l[i]));
           }
         } else {
-          const bool is_head = it.began && !it.open && piece_end < use.end;      // more pieces follow
-          float* dst = is_head ? p.head + (static_cast<long>(blockIdx.x) * S::kGroups + grp) * S::kRows * D : reinterpret_cast<float*>(ring);
+          const bool is_head = it.began && !it.open && piece_end < use.end;                // more pieces follow
+          float* dst = is_head ? p.head + (static_cast<long>(blockIdx.x) * kWarps + warp) * R * D : reinterpret_cast<float*>(ring);
           int* item = is_head ? left.head_item : left.tail_item;
           item[0] = it.b;
           item[1] = it.h;
           item[2] = it.row0;
           if (is_head) {
             left.head = 1;
-          } else {
+          } else {                                                     // (the sums go where the ring was)
             left.tail = 1;
             left.began = it.began;
             left.open = it.open;
             left.tail_end = it.item_end;
-            // the sums go where the ring is: every warp of the worker has let go of its last tiles
-            if (MT > 1)
-              for (int i = 0; i < S::kSlots; ++i) {                      // a slot's last round: this one before `slot`, else the one before it
-                const uint32_t done = round + (i < slot);
-                if (done > 0) ok = ok && tc5::mbar_wait_warp(&sm.empty[grp][i], (done - 1) & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_EMPTY);
-              }
+            __syncwarp();
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int row = mt * 16 + r + 8 * i;
-            if ((lane & 3) == 0) sm.ml[grp][is_head ? 0 : 1][row] = make_float2(w.m[i], w.l[i]);
-#pragma unroll
-            for (int d = 0; d < D / 8; ++d)
-              *reinterpret_cast<float2*>(dst + row * D + d * 8 + col) = make_float2(w.o[d][2 * i], w.o[d][2 * i + 1]);
+            if (w.writes_sums()) sm.ml[warp][is_head ? 0 : 1][w.row(i)] = make_float2(w.m[i], w.l[i]);
+            w.store(dst + w.row(i) * D, i);
           }
         }
       }
       held = more;
       if (!more) break;
       it = use.p;
-      row0 = it.row0 + mt * 16;
       fresh = true;
       w.clear();
-      // positions of the warp's first and last row
+      // positions of the lane's two rows, and of the first and last one
       const int rows = it.n * p.G;
-      p0 = row0 < rows ? it.past + token_of(p, row0) : -1;
-      p1 = row0 < rows ? it.past + token_of(p, min(row0 + 15, rows - 1)) : -1;
-      full = row0 + 15 < rows;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = token_of(p, it.row0 + w.row(i));
+        w.pos[i] = at < it.n ? it.past + at : -1;
+      }
+      p0 = it.past + token_of(p, it.row0);
+      p1 = it.past + token_of(p, min(it.row0 + R, rows) - 1);
+      full = it.row0 + R <= rows;
       u2 = 2 * it.lo;
       u2_end = 2 * it.hi;
     }
@@ -654,27 +797,24 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
       start = false;
       continue;
     }
-    ok = ok && held && tc5::mbar_wait_warp(&sm.full[grp][slot], round & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_FULL);
+    ok = ok && held && tc5::mbar_wait_warp(&sm.full[warp][slot], round & 1, &sm.abort_flag, p.status, STATUS_TIMEOUT_SMEM_FULL);
     if (!ok) break;
     if (fresh) {
-      w.take(raw, p.scale);
+      w.take(p.scale);
       fresh = false;
     }
     const int key0 = (u2 >> 1) * 64;
     if (key0 <= p1 && (p.window == 0 || key0 + 63 > p0 - p.window)) {
       if (u2 & 1) {
-        accumulate<D, S>(w, ring + slot * S::kSlot, pr);
+        w.values(ring + slot * S::kSlot);
         if ((u2 & 7) == 7) w.settle();
       } else {
-        const float2 scale = sm.scale[grp][slot][lane & 3];
-        float s[8][4];
-        scores<D, S>(w, ring + slot * S::kSlot, s);
+        const float2 scale = sm.scale[warp][slot][w.sub_block()];
         const bool whole = full && key0 + 63 <= p0 && (p.window == 0 || key0 > p1 - p.window);
-        softmax<D>(w, s, pr, scale, !whole || __any_sync(0xffffffffu, scale.x == 0.f), key0 + 16 * (lane & 3), p.window);
+        w.keys(ring + slot * S::kSlot, scale, !whole || __any_sync(0xffffffffu, scale.x == 0.f), key0 + 16 * w.sub_block(), p.window);
       }
     }
     __syncwarp();
-    if (MT > 1 && lane == 0) tc5::mbar_arrive(&sm.empty[grp][slot]);
     if (++slot == S::kSlots) {
       slot = 0;
       ++round;
@@ -682,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
     ++u2;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  if (mt == 0 && lane == 0) sm.left[grp] = left;
+  if (lane == 0) sm.left[warp] = left;
   __syncthreads();
   if (sm.abort_flag) {
     if (tid == 0) p.join[blockIdx.x].any = 0;
@@ -690,8 +830,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
   }
 
   // ---- parts of one item in several workers meet; those of an item that goes beyond the CTA are left for the join
-  const Left mine = sm.left[lane < S::kGroups ? lane : 0];
-  const bool is = lane < S::kGroups;
+  const Left mine = sm.left[lane < kWarps ? lane : 0];
+  const bool is = lane < kWarps;
   const unsigned some = __ballot_sync(0xffffffffu, is && mine.some), heads = __ballot_sync(0xffffffffu, is && mine.head);
   const unsigned tails = __ballot_sync(0xffffffffu, is && mine.tail), began = __ballot_sync(0xffffffffu, is && mine.tail && mine.began);
   const unsigned opens = __ballot_sync(0xffffffffu, is && mine.tail && mine.open);
@@ -699,9 +839,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
   // kGroups at the first worker's head.
   int g1 = is ? lane : 0;
   bool open = is && (opens >> lane & 1);
-  const bool chain = is ? (tails >> lane & 1) && (lane == 0 || !(began >> lane & 1)) : lane == S::kGroups && (heads & 1);
+  const bool chain = is ? (tails >> lane & 1) && (lane == 0 || !(began >> lane & 1)) : lane == kWarps && (heads & 1);
   unsigned from = is ? 0u : 1u;                                        // workers whose contribution is a head
-  while (open && g1 + 1 < S::kGroups && (some >> (g1 + 1) & 1)) {
+  while (open && g1 + 1 < kWarps && (some >> (g1 + 1) & 1)) {
     ++g1;
     from |= heads & (1u << g1);
     open = !(heads >> g1 & 1) && (opens >> g1 & 1);
@@ -718,24 +858,24 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
   // head.
   constexpr int kCols = D / 32;
   for (unsigned chains = __ballot_sync(0xffffffffu, chain); chains; chains &= chains - 1) {
-    const int which = __ffs(chains) - 1, first = which < S::kGroups ? which : 0, last = __shfl_sync(0xffffffffu, g1, which);
+    const int which = __ffs(chains) - 1, first = which < kWarps ? which : 0, last = __shfl_sync(0xffffffffu, g1, which);
     const bool closed = __shfl_sync(0xffffffffu, static_cast<int>(from != 0), which);              // by a head
     const bool began_before = __shfl_sync(0xffffffffu, static_cast<int>(before), which), ends = !__shfl_sync(0xffffffffu, static_cast<int>(open), which);
-    const int* item = which < S::kGroups ? sm.left[first].tail_item : sm.left[first].head_item;
+    const int* item = which < kWarps ? sm.left[first].tail_item : sm.left[first].head_item;
     const Request rq = sm.request[item[0]];
     const int stop = last + !closed;                                   // tails: first .. stop - 1
-    const float* head = p.head + (static_cast<long>(blockIdx.x) * S::kGroups + last) * S::kRows * D;
-    const long part = (static_cast<long>(blockIdx.x) * 2 + (began_before ? 0 : 1)) * S::kRows;
+    const float* head = p.head + (static_cast<long>(blockIdx.x) * kWarps + last) * R * D;
+    const long part = (static_cast<long>(blockIdx.x) * 2 + (began_before ? 0 : 1)) * R;
 #pragma unroll 2
-    for (int row = warp; row < S::kRows; row += kWarps) {
-      float2 x[S::kGroups + 1][kCols / 2], ml[S::kGroups + 1];
+    for (int row = warp; row < R; row += kWarps) {
+      float2 x[kWarps + 1][kCols / 2], ml[kWarps + 1];
       const int at = row * D + lane * 2;
-      ml[S::kGroups] = closed ? sm.ml[last][0][row] : make_float2(-CUDART_INF_F, 0.f);
+      ml[kWarps] = closed ? sm.ml[last][0][row] : make_float2(-CUDART_INF_F, 0.f);
 #pragma unroll
       for (int c = 0; c < kCols / 2; ++c)
-        x[S::kGroups][c] = closed ? *reinterpret_cast<const float2*>(head + at + c * 64) : make_float2(0.f, 0.f);
+        x[kWarps][c] = closed ? *reinterpret_cast<const float2*>(head + at + c * 64) : make_float2(0.f, 0.f);
 #pragma unroll
-      for (int g = 0; g < S::kGroups; ++g) {
+      for (int g = 0; g < kWarps; ++g) {
         const bool in = g >= first && g < stop;
         ml[g] = in ? sm.ml[g][1][row] : make_float2(-CUDART_INF_F, 0.f);
 #pragma unroll
@@ -744,11 +884,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
       }
       float m = -CUDART_INF_F, l = 0.f;
 #pragma unroll
-      for (int g = 0; g <= S::kGroups; ++g) m = fmaxf(m, ml[g].x);
+      for (int g = 0; g <= kWarps; ++g) m = fmaxf(m, ml[g].x);
       const float ref = m == -CUDART_INF_F ? 0.f : m;
       float2 o[kCols / 2] = {};
 #pragma unroll
-      for (int g = 0; g <= S::kGroups; ++g) {
+      for (int g = 0; g <= kWarps; ++g) {
         const float f = ex2(ml[g].x - ref);
         l = fmaf(ml[g].y, f, l);
 #pragma unroll
@@ -771,16 +911,15 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
 
 // Parts of items that several CTAs worked on: CTA (c, part) takes some rows of the item that begins in CTA c of the kernel before.
 constexpr int kJoinParts = 4;
-template <int D, int MT>
+template <int D, int R>
 __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int kRows = 16 * MT;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x;
   const Join j = p.join[c];
   if (!j.any) return;
-  const int last = static_cast<int>((j.end - 1) / j.each / (kWarps / MT));
-  for (int e = blockIdx.y * 128 + threadIdx.x; e < kRows * (D / 4); e += kJoinParts * 128) {
+  const int last = static_cast<int>((j.end - 1) / j.each / kWarps);
+  for (int e = blockIdx.y * 128 + threadIdx.x; e < R * (D / 4); e += kJoinParts * 128) {
     const int row = e / (D / 4), d = (e % (D / 4)) * 4;
     bf16* out = row_of(p, j.n, j.q0, j.h, j.row0 + row, D);
     if (!out) continue;
@@ -792,7 +931,7 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_const
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int g = min(g0 + i, last);
-        const long slot = (static_cast<long>(g) * 2 + (g == c)) * kRows + row;
+        const long slot = (static_cast<long>(g) * 2 + (g == c)) * R + row;
         ml[i] = p.part_ml[slot];
         x[i] = *reinterpret_cast<const float4*>(p.part + slot * D + d);
         if (g0 + i > last) ml[i] = make_float2(-CUDART_INF_F, 0.f);
@@ -821,18 +960,18 @@ __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_const
   }
 }
 
-template <int D, int MT>
+template <int D, int R>
 cudaError_t run(const AttnParams& p, int grid, cudaStream_t st) {
-  constexpr int bytes = sizeof(Smem<D, MT>);
+  constexpr int bytes = sizeof(Smem<D, R>);
   static_assert(bytes <= 232448, "shared memory of one CTA");
   int dev = 0;
   cudaGetDevice(&dev);
   static std::atomic<unsigned long long> ready{0};                     // devices on which the kernel may have this much shared memory
   cudaError_t e = cudaSuccess;
   if (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    e = cudaFuncSetAttribute(cache_attn_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    e = cudaFuncSetAttribute(cache_attn_kernel<D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     // the same division of shared memory for the join: an SM changes it only when it is empty
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(cache_attn_join_kernel<D, MT>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(cache_attn_join_kernel<D, R>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
     if (dev <= 63) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
@@ -846,24 +985,26 @@ cudaError_t run(const AttnParams& p, int grid, cudaStream_t st) {
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, MT>, p);
+  e = cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, R>, p);
   if (e != cudaSuccess) return e;
   cfg.gridDim = dim3(grid, kJoinParts);
   cfg.blockDim = 128;
   cfg.dynamicSmemBytes = 0;
-  e = cudaLaunchKernelEx(&cfg, cache_attn_join_kernel<D, MT>, p);
+  e = cudaLaunchKernelEx(&cfg, cache_attn_join_kernel<D, R>, p);
   nsa::count_launch(2);
   return e;
 }
 
-// Warps on the same keys: rows of a request over 16, up to 8
-int row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
+// Rows of a tile: 8 where a request's queries of one KV head are that many at most (16 heads of 128 on 2, 16 contexts of 16000 tokens: 22.2 us, with 16 28.0), else
+// 16.  More rows are more tiles, each with its own pass over the keys, which L2 holds for the next one: two, four or eight warps with a tile each on the
+// same copies were slower (32 rows 125 -> 170 us, 64 rows 42 -> 69, 128 rows 130 -> 202), since they wait for one another.
+int tile_rows(long rows) { return rows <= 8 ? 8 : 16; }
 }  // namespace
 
 // Floats of scratch that nsa_cache_attention needs
 extern "C" long nsa_cache_attention_scratch(int Hq, int H, int D, int max_new) {
-  const long G = H > 0 ? Hq / H : 1, mt = row_tiles(static_cast<int>(G * max_new < 1024 ? G * max_new : 1024)), grid = nsa::sm_count(), rows = 16 * mt;
-  return grid * (kWarps / mt) * rows * D + grid * 2 * rows * (D + 2) + grid * static_cast<long>(sizeof(Join) / 4);
+  const long grid = nsa::sm_count(), rows = tile_rows(static_cast<long>(H > 0 ? Hq / H : 1) * max_new);
+  return grid * kWarps * rows * D + grid * 2 * rows * (D + 2) + grid * static_cast<long>(sizeof(Join) / 4);
 }
 
 extern "C" int nsa_cache_attention(const void* q, long ldq, const void* kc, const void* vc, const float* scale, const int* table, const int* query_start,
@@ -883,8 +1024,7 @@ extern "C" int nsa_cache_attention(const void* q, long ldq, const void* kc, cons
   p.window = window;
   p.scale = softmax_scale * 1.4426950408889634f;
   p.status = nsa::status_ptr();
-  const long most = static_cast<long>(p.G) * max_new;
-  const int mt = row_tiles(static_cast<int>(most < 1024 ? most : 1024)), grid = nsa::sm_count(), rows = 16 * mt;
+  const int grid = nsa::sm_count(), rows = tile_rows(static_cast<long>(p.G) * max_new);
   p.part = scratch;
   p.part_ml = reinterpret_cast<float2*>(p.part + static_cast<long>(grid) * 2 * rows * D);
   p.join = reinterpret_cast<Join*>(p.part_ml + static_cast<long>(grid) * 2 * rows);
@@ -893,9 +1033,9 @@ extern "C" int nsa_cache_attention(const void* q, long ldq, const void* kc, cons
   for (int b = 0; b < B && e == cudaSuccess; b += kMaxRequests) {      // a launch for each 768 requests, on the same scratch
     p.s = CacheStep{table + static_cast<long>(b) * W, query_start + b, lengths + b, B - b < kMaxRequests ? B - b : kMaxRequests, W, N};
     if (D == 128)
-      e = mt == 1 ? run<128, 1>(p, grid, st) : mt == 2 ? run<128, 2>(p, grid, st) : mt == 4 ? run<128, 4>(p, grid, st) : run<128, 8>(p, grid, st);
+      e = rows == 8 ? run<128, 8>(p, grid, st) : run<128, 16>(p, grid, st);
     else
-      e = mt == 1 ? run<64, 1>(p, grid, st) : mt == 2 ? run<64, 2>(p, grid, st) : mt == 4 ? run<64, 4>(p, grid, st) : run<64, 8>(p, grid, st);
+      e = rows == 8 ? run<64, 8>(p, grid, st) : run<64, 16>(p, grid, st);
   }
   return e == cudaSuccess ? 0 : nsa::fail_cuda(e, "nsa_cache_attention launch");
 }
