@@ -198,6 +198,7 @@ struct Smem {
   Sums all;
   short list[kThreads], rest[kThreads];    // threads of which four pieces, or all, are looked at again
   u64 buffer[kBuffer];
+  uint4 piece[4][33];                      // of lanes, where their hits are read by number
   u64 best[kTopMax];
   uint64_t full[kStages], empty[kStages];
   int abort_flag;
@@ -355,14 +356,17 @@ __device__ __noinline__ void select(Smem& sm, const Part<T>& p, int b, int k) {
       if (j[i] < 0) hits &= ~(((1u << kN) - 1) << (i * kN));
     }
     if (none) hits = 0;
+    if (!__any_sync(kAll, hits)) return;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) sm.piece[i][lane] = *reinterpret_cast<const uint4*>(&v[i].w);
 #pragma unroll 1
-    while (__any_sync(kAll, hits)) {                                   // one of each lane's; the number is read again, from L1
+    while (__any_sync(kAll, hits)) {                                   // one of each lane's
       const int at = hits ? __ffs(hits) - 1 : 0;
       int piece = j[0];
 #pragma unroll
       for (int i = 1; i < kAtOnce; ++i) piece = at / kN == i ? j[i] : piece;
-      const int col = p.base + piece * kN + at % kN;
-      candidate(hits != 0, hits ? value(p.x, col) : 0.f, col);
+      candidate(hits != 0, value(reinterpret_cast<const T*>(&sm.piece[at / kN][lane]), at % kN), p.base + piece * kN + at % kN);
       hits &= hits - 1;
     }
   };
@@ -489,16 +493,11 @@ __device__ __noinline__ void finish(Smem& sm, Sums a, const T* x, long row, long
   u64 head = lane < parts ? sm.buffer[lane * k] : 0, mine = 0;
 #pragma unroll 1
   for (int place = 0; place < k; ++place) {
-    u64 r = head;
-#pragma unroll
-    for (int o = 4; o; o >>= 1) {
-      const u64 a = __shfl_xor_sync(0xffffffffu, r, o);
-      r = a > r ? a : r;
-    }
-    r = __shfl_sync(0xffffffffu, r, 0);
-    if (lane == place) mine = r;
-    if (head == r && lane < parts) {
-      head = next < k ? sm.buffer[lane * k + next] : 0;
+    const unsigned high = static_cast<unsigned>(head >> 32), low = static_cast<unsigned>(head), best = __reduce_max_sync(0xffffffffu, high);
+    const unsigned first = __reduce_max_sync(0xffffffffu, high == best ? low : 0u);
+    if (lane == place) mine = static_cast<u64>(best) << 32 | first;
+    if (high == best && low == first) {                                // one lane's: ranks differ (but for those of lanes without a part, 0)
+      head = next < k && lane < parts ? sm.buffer[lane * k + next] : 0;
       ++next;
     }
   }
@@ -604,6 +603,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) logprobs_fwd_kernel(cons
         Sums a = sm.all;
         if (parts > 1) {                                               // lane c fetches part c's
           const Sums o = *cg::this_cluster().map_shared_rank(&sm.all, lane < parts ? lane : 0);
+#pragma unroll 1
           for (int c = 1; c < parts; ++c)
             a.add(Sums{__shfl_sync(0xffffffffu, o.m, c), __shfl_sync(0xffffffffu, o.R, c), __shfl_sync(0xffffffffu, o.S, c), __shfl_sync(0xffffffffu, o.E, c)});
         }
