@@ -401,48 +401,64 @@ __global__ void __maxnreg__(80) cache_append_kernel(const bf16* __restrict__ k, 
   }
 }
 
-// One CTA per page and head: bf16 values (n, P, H, D) of both sides.  Keys 16 codes of a token at a time; values 16 tokens of C columns, so that a warp's
-// stores are whole rows.  Bytes bound it.  XX
+// One CTA per page, head and side: bf16 values (n, P, H, D).  Keys 8 codes of a token at a time, four such loads before the first store; values 16 tokens of
+// C columns, so that a warp's stores are whole rows.  Bytes bound it.  XX
+__device__ __forceinline__ float number_of(uint32_t w, int i, float s) {   // (code i of a word - 128) s, s a power of two: 2^23 + u by its bits
+  return fmaf(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)), s, -8388736.f * s);
+}
+__device__ __forceinline__ uint32_t two_of(float a, float b) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 template <int C>
 __global__ void __launch_bounds__(128) cache_values_kernel(CachePages c, const int* __restrict__ ids, bf16* __restrict__ k, bf16* __restrict__ v) {
   const int h = blockIdx.y, P = 1 << c.shift, D = c.D, page = ids[blockIdx.x], t = threadIdx.x, lane = t & 31;
   const bool there = page >= 0 && page < c.pages;
   const long ph = static_cast<long>(there ? page : 0) * c.H + h, row = static_cast<long>(c.H) * D, out = static_cast<long>(blockIdx.x) * P * row + h * D;
-  const float2 scale = *reinterpret_cast<const float2*>(c.scale + ph * 2);
-  auto two = [](uint32_t w, int i, float s) {                          // codes i and i + 1 of a word
-    const __nv_bfloat162 r = __floats2bfloat162_rn((static_cast<float>(w >> (8 * i) & 0xff) - 128.f) * s, (static_cast<float>(w >> (8 * i + 8) & 0xff) - 128.f) * s);
-    return *reinterpret_cast<const uint32_t*>(&r);
-  };
-  const uint8_t* kc = c.k + ph * P * D;
-  for (int y = t * 16; y < P * D; y += 128 * 16) {
-    const int token = y / (2 * D) * 2 + (y >> 6 & 1), d = (y % (2 * D) >> 7) * 64 + (y & 63);
-    const uint4 w = there ? *reinterpret_cast<const uint4*>(kc + y) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-    const float s = there ? scale.x : 0.f;
-    uint4* to = reinterpret_cast<uint4*>(k + out + token * row + d);
-    to[0] = make_uint4(two(w.x, 0, s), two(w.x, 2, s), two(w.y, 0, s), two(w.y, 2, s));
-    to[1] = make_uint4(two(w.z, 0, s), two(w.z, 2, s), two(w.w, 0, s), two(w.w, 2, s));
+  const float s = there ? c.scale[ph * 2 + blockIdx.z] : 0.f;
+  if (blockIdx.z == 0) {
+    const uint8_t* codes = c.k + ph * P * D;
+    for (int y0 = t * 8; y0 < P * D; y0 += 4 * 128 * 8) {
+      uint2 w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int y = y0 + j * 128 * 8;
+        w[j] = there && y < P * D ? __ldg(reinterpret_cast<const uint2*>(codes + y)) : make_uint2(0x80808080u, 0x80808080u);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int y = y0 + j * 128 * 8, token = y / (2 * D) * 2 + (y >> 6 & 1), d = (y % (2 * D) >> 7) * 64 + (y & 63);
+        if (y >= P * D) break;
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = i < 2 ? w[j].x : w[j].y;
+          o[i] = two_of(number_of(u, 2 * (i & 1), s), number_of(u, 2 * (i & 1) + 1, s));
+        }
+        *reinterpret_cast<uint4*>(k + out + token * row + d) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+    return;
   }
-  const uint8_t* vc = c.v + ph * P * D;
+  const uint8_t* codes = c.v + ph * P * D;
   const int slabs = D / (32 * C);
-  const float s = there ? scale.y : 0.f;
   for (int y = t >> 5; y < P / 16 * slabs; y += 4) {
     const int t0 = y / slabs * 16, d = (y % slabs) * 32 * C + lane * C;
     uint32_t w[C][4];
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const uint4 u = there ? *reinterpret_cast<const uint4*>(vc + value_at(t0, d + i, D)) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+      const uint4 u = there ? __ldg(reinterpret_cast<const uint4*>(codes + value_at(t0, d + i, D))) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
       w[i][0] = u.x;
       w[i][1] = u.y;
       w[i][2] = u.z;
       w[i][3] = u.w;
     }
-    auto number = [&](int i, int tok) { return (static_cast<float>(w[i][tok >> 2] >> (8 * (tok & 3)) & 0xff) - 128.f) * s; };
 #pragma unroll
     for (int tok = 0; tok < 16; ++tok) {
       bf16* to = v + out + (t0 + tok) * row + d;
-      const __nv_bfloat162 a = __floats2bfloat162_rn(number(0, tok), number(1, tok)), b = __floats2bfloat162_rn(number(C - 2, tok), number(C - 1, tok));
-      if (C == 4) *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-      else *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(&a);
+      const uint32_t a = two_of(number_of(w[0][tok >> 2], tok & 3, s), number_of(w[1][tok >> 2], tok & 3, s));
+      if (C == 4) *reinterpret_cast<uint2*>(to) = make_uint2(a, two_of(number_of(w[C - 2][tok >> 2], tok & 3, s), number_of(w[C - 1][tok >> 2], tok & 3, s)));
+      else *reinterpret_cast<uint32_t*>(to) = a;
     }
   }
 }
@@ -506,9 +522,9 @@ extern "C" int nsa_cache_values(const void* kc, const void* vc, const float* sca
   const CachePages c{static_cast<uint8_t*>(const_cast<void*>(kc)), static_cast<uint8_t*>(const_cast<void*>(vc)), const_cast<float*>(scale), pages, H, D,
                      __builtin_ctz(page_size)};
   if (D % 128)
-    cache_values_kernel<2><<<dim3(n, H), 128, 0, st>>>(c, ids, static_cast<bf16*>(k), static_cast<bf16*>(v));
+    cache_values_kernel<2><<<dim3(n, H, 2), 128, 0, st>>>(c, ids, static_cast<bf16*>(k), static_cast<bf16*>(v));
   else
-    cache_values_kernel<4><<<dim3(n, H), 128, 0, st>>>(c, ids, static_cast<bf16*>(k), static_cast<bf16*>(v));
+    cache_values_kernel<4><<<dim3(n, H, 2), 128, 0, st>>>(c, ids, static_cast<bf16*>(k), static_cast<bf16*>(v));
   nsa::count_launch();
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : nsa::fail_cuda(e, "nsa_cache_values launch");

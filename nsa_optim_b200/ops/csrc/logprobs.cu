@@ -33,7 +33,8 @@ constexpr int kCtas = 5;                  // per SM
 constexpr int kUnroll = 4, kHalves = 2;   // 16-byte pieces of a thread at a time; of a chunk
 constexpr int kChunk = kThreads * kUnroll * kHalves, kStages = 2;      // pieces that a bulk copy brings (16 KB); chunks on their way or in use
 constexpr int kTopMax = 32;               // tokens that the selection gives
-constexpr int kBuffer = 512;              // candidates for them
+constexpr int kBuffer = 480;              // candidates for them
+constexpr int kParts = 8;                 // CTAs of a cluster
 constexpr int kWidest = 32767 * kThreads * kUnroll * 4;      // columns: halves of chunks are counted in 16 bits
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLow = -1e30f;            // logits below it count as this in the pass: 2^-inf times -inf is no number
@@ -194,8 +195,11 @@ struct Smem {
   alignas(16) unsigned other[2][kThreads]; // of the pieces that do not lie with it
   alignas(8) short where[2][kThreads];     // the chunk half that it lies in; -1: a piece that is not whole
   uint64_t ready[2], taken[2];
-  // the fifth warp's
-  Sums all;
+  // what the cluster's CTAs leave here
+  Sums all[kParts];
+  u64 lists[kParts][kTopMax];
+  // of the warp of the rows' ends
+  alignas(16) uint2 pairs[32];
   short list[kThreads], rest[kThreads];    // threads of which four pieces, or all, are looked at again
   u64 buffer[kBuffer];
   uint4 piece[4][33];                      // of lanes, where their hits are read by number
@@ -209,6 +213,15 @@ __device__ __forceinline__ void warp_reduce(Sums& s) {                 // lanes 
     s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
     s.E += __shfl_xor_sync(0xffffffffu, s.E, o);
   }
+}
+
+// Of n lanes that lie together, n a power of two: in all of them
+__device__ __forceinline__ Sums join(Sums s, int n) {
+#pragma unroll 1
+  for (int o = n >> 1; o; o >>= 1)
+    s.add(Sums{__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.R, o), __shfl_xor_sync(0xffffffffu, s.S, o),
+               __shfl_xor_sync(0xffffffffu, s.E, o)});
+  return s;
 }
 
 // The sums of a part and the thread's own maximum.  get: chunks that the CTA has read
@@ -273,7 +286,7 @@ __device__ __forceinline__ Sums pass(const Part<T>& p, Smem& sm, const uint4* ri
     }
   }
   // the first and the last piece, where they are not whole
-  if (threadIdx.x < 64) {
+  if (threadIdx.x < 64 && (p.w0 == 1 || p.w1 < p.pieces)) {
     float2 x[kN / 2];
     float m = -CUDART_INF_F;
     const int j = p.odd_piece(threadIdx.x);
@@ -302,16 +315,18 @@ __device__ __noinline__ void select(Smem& sm, const Part<T>& p, int b, int k) {
   const int lane = threadIdx.x & 31, have = min(k, p.hi - p.lo);
   const uint4 four = *reinterpret_cast<const uint4*>(sm.top[b] + lane * 4), others = *reinterpret_cast<const uint4*>(sm.other[b] + lane * 4);
   const unsigned mine[kEach] = {four.x, four.y, four.z, four.w}, second[kEach] = {others.x, others.y, others.z, others.w};
-  // the have-th largest of the pairs: the largest of all is taken out so many times (no logit's order is 0)
-  unsigned g0 = max(four.x, four.y), g1 = max(four.z, four.w), kth = 0;
-#pragma unroll 1
-  for (int n = 0; n < have; ++n) {
-    const unsigned m = max(g0, g1);
-    kth = __reduce_max_sync(kAll, m);
-    if (__ffs(__ballot_sync(kAll, m == kth)) - 1 == lane) {
-      if (g0 == kth) g0 = 0; else g1 = 0;
-    }
+  // the have-th largest of the pairs: the smallest of those with fewer than so many larger ones
+  const unsigned g0 = max(four.x, four.y), g1 = max(four.z, four.w);
+  int before0 = 0, before1 = 0;
+  sm.pairs[lane] = make_uint2(g0, g1);
+  __syncwarp();
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const uint4 o = reinterpret_cast<const uint4*>(sm.pairs)[i];
+    before0 += (o.x > g0) + (o.y > g0) + (o.z > g0) + (o.w > g0);
+    before1 += (o.x > g1) + (o.y > g1) + (o.z > g1) + (o.w > g1);
   }
+  const unsigned kth = __reduce_min_sync(kAll, min(before0 < have ? g0 : kAll, before1 < have ? g1 : kAll));
   int reach = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) reach += __popc(__ballot_sync(kAll, mine[i] >= kth));
@@ -341,68 +356,54 @@ __device__ __noinline__ void select(Smem& sm, const Part<T>& p, int b, int k) {
     if (is && at < kBuffer) sm.buffer[at] = rank_of(x, col);
     count += __popc(mask);
   };
-  constexpr int kAtOnce = 4;                                           // loads of a lane
-  auto look = [&](const Vec<T> (&v)[kAtOnce], const int (&j)[kAtOnce]) {                 // j: pieces, -1: none
-    unsigned hits = 0;
+  // A lane takes four pieces of a thread at a time: those of its largest logit, or four after four of all
+  const int turns = (p.w1 - p.w0 + kThreads - 1) / kThreads, fours = (turns + kUnroll - 1) / kUnroll, items = n + n_rest * fours;
+#pragma unroll 1
+  for (int e = lane; e - lane < items; e += 32) {
+    int who = -1, four = 0;
+    if (e < n) {
+      who = sm.list[e];
+      four = sm.where[b][who];
+    } else if (e < items) {
+      who = sm.rest[(e - n) / fours];
+      four = (e - n) % fours;
+    }
+    const int j0 = p.w0 + who + four * (kUnroll * kThreads), there = who < 0 || four < 0 ? 0 : min((p.w1 - j0 + kThreads - 1) / kThreads, kUnroll);
+    __syncwarp();
+    {
+      Vec<T> v[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
+      for (int i = 0; i < kUnroll; ++i)
+        if (i < there) v[i] = load(p.x + p.base + (j0 + i * kThreads) * kN);
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i)
+        if (i < there) sm.piece[i][lane] = *reinterpret_cast<const uint4*>(&v[i].w);
+    }
+    __syncwarp();
+    unsigned hits = 0;
+#pragma unroll 1
+    for (int i = 0; i < there; ++i) {
+      Vec<T> v;
       float2 x[kN / 2];
-      v[i].exact(x);
+      *reinterpret_cast<uint4*>(&v.w) = sm.piece[i][lane];
+      v.exact(x);
+      unsigned some = 0;
 #pragma unroll
       for (int c = 0; c < kN / 2; ++c) {
-        if (!(x[c].x <= under)) hits |= 1u << (i * kN + 2 * c);
-        if (!(x[c].y <= under)) hits |= 2u << (i * kN + 2 * c);
+        if (!(x[c].x <= under)) some |= 1u << (2 * c);
+        if (!(x[c].y <= under)) some |= 2u << (2 * c);
       }
-      if (j[i] < 0) hits &= ~(((1u << kN) - 1) << (i * kN));
+      hits |= some << (i * kN);
     }
     if (none) hits = 0;
-    if (!__any_sync(kAll, hits)) return;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) sm.piece[i][lane] = *reinterpret_cast<const uint4*>(&v[i].w);
 #pragma unroll 1
     while (__any_sync(kAll, hits)) {                                   // one of each lane's
       const int at = hits ? __ffs(hits) - 1 : 0;
-      int piece = j[0];
-#pragma unroll
-      for (int i = 1; i < kAtOnce; ++i) piece = at / kN == i ? j[i] : piece;
-      candidate(hits != 0, value(reinterpret_cast<const T*>(&sm.piece[at / kN][lane]), at % kN), p.base + piece * kN + at % kN);
+      candidate(hits != 0, value(reinterpret_cast<const T*>(&sm.piece[at / kN][lane]), at % kN), p.base + (j0 + at / kN * kThreads) * kN + at % kN);
       hits &= hits - 1;
     }
-  };
-  // the four pieces of a thread's largest logit: a lane takes those of one thread
-#pragma unroll 1
-  for (int e = 0; e < n; e += 32) {
-    Vec<T> v[kAtOnce];
-    int j[kAtOnce];
-    const int who = e + lane < n ? sm.list[e + lane] : 0, half = e + lane < n ? sm.where[b][who] : -1;
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      j[i] = p.w0 + who + (half * kUnroll + i) * kThreads;
-      if (half < 0 || j[i] >= p.w1) j[i] = -1;
-      v[i].clear();
-      if (j[i] >= 0) v[i] = load(p.x + p.base + j[i] * kN);
-    }
-    look(v, j);
   }
-  // all pieces of the others
-  const int turns = (p.w1 - p.w0 + kThreads - 1) / kThreads;
-#pragma unroll 1
-  for (int e = 0; e < n_rest; ++e)
-#pragma unroll 1
-    for (int turn = 0; turn < turns; turn += 32 * kAtOnce) {
-      Vec<T> v[kAtOnce];
-      int j[kAtOnce];
-#pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        j[i] = p.w0 + sm.rest[e] + (turn + i * 32 + lane) * kThreads;
-        if (j[i] >= p.w1) j[i] = -1;
-        v[i].clear();
-        if (j[i] >= 0) v[i] = load(p.x + p.base + j[i] * kN);
-      }
-      look(v, j);
-    }
-  {                                                                    // the pieces that are not whole: a column per lane
+  if (p.w0 == 1 || p.w1 < p.pieces) {                                  // pieces that are not whole: a column per lane
     const int j = p.odd_piece(lane < kN ? 0 : 32), col = p.base + j * kN + lane % kN;
     const float x = j >= 0 && lane < 2 * kN ? p.at(col) : -CUDART_INF_F;
     candidate(j >= 0 && lane < 2 * kN && ordered(x) > bound, x, col);
@@ -443,10 +444,10 @@ __device__ __noinline__ void select(Smem& sm, const Part<T>& p, int b, int k) {
   __syncwarp();
 }
 
-// A row's end, by one warp: a are its sums, sm.best of the cluster's CTAs its candidates.
+// A row's end, by one warp of each CTA: a are the row's sums, lists its parts' best in order.  Each CTA places its own, the first one writes the rest.
 template <class T>
-__device__ __noinline__ void finish(Smem& sm, Sums a, const T* x, long row, long long tok, float chosen, float* logprob, float* entropy, float2* stats, float* top_out,
-                                    long long* index, int V, int k, long long ignore, int parts, KernelStatus* status) {
+__device__ __noinline__ void finish(const u64* lists, Sums a, const T* x, long row, long long tok, float chosen, float* logprob, float* entropy, float2* stats, float* top_out,
+                                    long long* index, int V, int k, long long ignore, int part, int parts, KernelStatus* status) {
   const int lane = threadIdx.x & 31;
   float m = a.m, logS = logf(a.S) - fmaf(m, kLog2e, -a.R) * kLn2, H = logf(a.S);
   bool empty = false;
@@ -466,46 +467,40 @@ __device__ __noinline__ void finish(Smem& sm, Sums a, const T* x, long row, long
     H = logS = empty ? 0.f : logf(a.S);
   }
   H = empty ? 0.f : H - a.E * kLn2 / a.S;
-  if (lane == 0) {
+  if (lane == 0 && part == 0) {
     NSA_CHECK_INDEX(tok == ignore || (tok >= 0 && tok < V), status, tok);
     logprob[row] = tok == ignore || tok < 0 || tok >= V ? 0.f : empty ? m : chosen - m - logS;
     entropy[row] = H;
     stats[row] = make_float2(m, logS);                                 // apart: their sum would round a probability by |m| 2^-24
   }
   if (k == 0) return;
-  auto put = [&](int place, u64 r) {
-    index[row * k + place] = index_of(r);
-    top_out[row * k + place] = empty ? m : logit_of(r) - m - logS;
-  };
-  if (parts == 1) {
-    if (lane < k) put(lane, sm.best[lane]);
-    return;
-  }
-  // each part's best are in order: the best of their heads k times
-  const int n = parts * k;
-#pragma unroll
-  for (int i = 0; i < 8 * kTopMax / 32; ++i) {
-    const int at = i * 32 + lane;
-    if (at < n) sm.buffer[at] = *cg::this_cluster().map_shared_rank(&sm.best[at % k], at / k);
-  }
-  __syncwarp();
-  int next = 1;
-  u64 head = lane < parts ? sm.buffer[lane * k] : 0, mine = 0;
+  // a token's place is the number of larger ones in all lists: 32 ranks each, that of no token is 0
+  const u64 mine = lists[part * kTopMax + lane];
+  int place = lane;
+  if (parts > 1) {
+    int n[kParts] = {};
 #pragma unroll 1
-  for (int place = 0; place < k; ++place) {
-    const unsigned high = static_cast<unsigned>(head >> 32), low = static_cast<unsigned>(head), best = __reduce_max_sync(0xffffffffu, high);
-    const unsigned first = __reduce_max_sync(0xffffffffu, high == best ? low : 0u);
-    if (lane == place) mine = static_cast<u64>(best) << 32 | first;
-    if (high == best && low == first) {                                // one lane's: ranks differ (but for those of lanes without a part, 0)
-      head = next < k && lane < parts ? sm.buffer[lane * k + next] : 0;
-      ++next;
-    }
+    for (int step = kTopMax / 2; step; step >>= 1)
+#pragma unroll
+      for (int c = 0; c < kParts; ++c)
+        if (c < parts) n[c] += lists[c * kTopMax + n[c] + step - 1] > mine ? step : 0;
+    place = 0;
+#pragma unroll
+    for (int c = 0; c < kParts; ++c)
+      if (c < parts) place += n[c] + (lists[c * kTopMax + n[c]] > mine);
   }
-  if (lane < k) put(lane, mine);
+  if (mine != 0 && place < k) {
+    index[row * k + place] = index_of(mine);
+    top_out[row * k + place] = empty ? m : logit_of(mine) - m - logS;
+  }
   __syncwarp();
 }
 
-// A cluster takes a row at a time, its CTAs even parts of the columns.
+// Of all threads of a cluster's CTAs: what came before their arrival is seen behind the wait, and an arrival follows the wait for the one before it
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// A CTA takes a row at a time; or a cluster its only one, each CTA an even part of the columns.
 template <class T>
 __global__ void __launch_bounds__(kThreads + 64, kCtas) logprobs_fwd_kernel(const T* __restrict__ logits, long ld, const long long* __restrict__ tokens,
                                                                             float* __restrict__ logprob, float* __restrict__ entropy,
@@ -530,6 +525,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) logprobs_fwd_kernel(cons
     tc5::fence_barrier_init();
   }
   __syncthreads();
+  if (parts > 1) cluster_arrive();                                     // the CTA runs: its memory may be written
   bool ok = true;
   uint32_t n = 0;                                                      // rows that this CTA has had
   if (warp < kWarps) {
@@ -547,10 +543,10 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) logprobs_fwd_kernel(cons
       sm.where[b][t] = static_cast<short>(where);
       if (lane == 0) sm.sums[b][warp] = s;
       tc5::arrive_warp(&sm.ready[b]);
-      if (parts > 1) {
-        cg::this_cluster().sync();
-        cg::this_cluster().sync();
-      }
+    }
+    if (parts > 1) {
+      cluster_wait();
+      cluster_arrive();
     }
   } else if (warp == kWarps) {                                         // the copies
     uint32_t put = 0;
@@ -570,10 +566,10 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) logprobs_fwd_kernel(cons
         }
       }
       __syncwarp();
-      if (parts > 1) {
-        cg::this_cluster().sync();
-        cg::this_cluster().sync();
-      }
+    }
+    if (parts > 1) {
+      cluster_wait();
+      cluster_arrive();
     }
     if (lane == 0 && sm.abort_flag)
       for (int i = 0; i < kStages; ++i) tc5::mbar_drain(&sm.full[i]);
@@ -592,24 +588,25 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) logprobs_fwd_kernel(cons
       // most of the time there is nothing to do: polling would take the others' issue slots
       for (int i = 0; i < 20000 && !__all_sync(0xffffffffu, tc5::mbar_try_wait(&sm.ready[b], n / 2 & 1)); ++i) __nanosleep(100);
       ok = ok && tc5::mbar_wait_warp(&sm.ready[b], n / 2 & 1, &sm.abort_flag, status, STATUS_TIMEOUT_SMEM_FULL);
+      Sums a{kLow, 0.f, 0.f, 0.f};
       if (ok) {
-        Sums a = sm.sums[b][0];
-        for (int w = 1; w < kWarps; ++w) a.add(sm.sums[b][w]);
-        sm.all = a;
+        a = join(sm.sums[b][lane % kWarps], kWarps);
         if (k > 0) select(sm, Part<T>(x, lo, hi), b, k);
       }
-      if (parts > 1) cg::this_cluster().sync();
-      if (part == 0 && ok) {
-        Sums a = sm.all;
-        if (parts > 1) {                                               // lane c fetches part c's
-          const Sums o = *cg::this_cluster().map_shared_rank(&sm.all, lane < parts ? lane : 0);
+      if (parts > 1) {
+        cluster_wait();
+        if (ok) {
+          if (lane < parts) *cg::this_cluster().map_shared_rank(&sm.all[part], lane) = a;
+          if (k > 0)
 #pragma unroll 1
-          for (int c = 1; c < parts; ++c)
-            a.add(Sums{__shfl_sync(0xffffffffu, o.m, c), __shfl_sync(0xffffffffu, o.R, c), __shfl_sync(0xffffffffu, o.S, c), __shfl_sync(0xffffffffu, o.E, c)});
+            for (int c = 0; c < parts; ++c) *cg::this_cluster().map_shared_rank(&sm.lists[part][lane], c) = sm.best[lane];
         }
-        finish(sm, a, x, row, tok, chosen, logprob, entropy, stats, top_out, index, V, k, ignore, parts, status);
+        cluster_arrive();
+        cluster_wait();
+        a = join(sm.all[lane & (parts - 1)], parts);                // a power of two
       }
-      if (parts > 1) cg::this_cluster().sync();                        // the others' memory is read until here
+      if (ok && (k > 0 || part == 0))
+        finish(parts > 1 ? sm.lists[0] : sm.best, a, x, row, tok, chosen, logprob, entropy, stats, top_out, index, V, k, ignore, part, parts, status);
       tc5::arrive_warp(&sm.taken[b]);
       tok = tok1;
       tok1 = tok2;
@@ -698,7 +695,7 @@ cudaError_t forward(const void* logits, long ld, const long long* tokens, float*
   // CTAs of a row: with fewer rows than SMs up to 8, of 4096 columns at least
   const int sms = nsa::sm_count();
   int parts = 1;
-  while (parts < 8 && rows * parts * 2 <= static_cast<long>(kCtas) * sms && V / (2 * parts) >= 4096) parts *= 2;
+  while (parts < kParts && rows * parts * 2 <= static_cast<long>(kCtas) * sms && V / (2 * parts) >= 4096) parts *= 2;
   cudaLaunchConfig_t cfg{};
   const long most = static_cast<long>(kCtas) * sms / parts;
   cfg.gridDim = static_cast<unsigned>((rows < most ? rows : most) * parts);
