@@ -196,17 +196,22 @@ __device__ __forceinline__ uint32_t coarser(uint32_t w, float ratio) {
   return bytes4(c[0], c[1], c[2], c[3]);
 }
 
-// The last request that begins at i or before, by a warp: 32 requests a load
-__device__ __forceinline__ int request_at(const int* start, int B, int i) {
+// The last request that begins at i or before, by a warp: 32 requests a load, of the last 31 all that is asked of them at once
+struct Request {
+  int b, first, next, length;
+};
+__device__ __forceinline__ Request request_at(const CacheStep& s, int i) {
   const int lane = threadIdx.x & 31;
-  int lo = 0, size = B;
-  while (size > 32) {
+  int lo = 0, size = s.B;
+  while (size > 31) {
     const int step = (size + 31) / 32, at = lo + lane * step;
-    const int n = __popc(__ballot_sync(0xffffffffu, at < lo + size && start[at] <= i));
+    const int n = __popc(__ballot_sync(0xffffffffu, at < lo + size && s.query_start[at] <= i));
     lo += max(n - 1, 0) * step;
-    size = min(step, B - lo);
+    size = min(step, s.B - lo);
   }
-  return lo + max(__popc(__ballot_sync(0xffffffffu, lane < size && start[lo + lane] <= i)) - 1, 0);
+  const int start = lane <= size ? s.query_start[lo + lane] : 0, length = lane < size ? s.lengths[lo + lane] : 0;
+  const int at = max(__popc(__ballot_sync(0xffffffffu, lane < size && start <= i)) - 1, 0);
+  return {lo + at, __shfl_sync(0xffffffffu, start, at), __shfl_sync(0xffffffffu, start, at + 1), __shfl_sync(0xffffffffu, length, at)};
 }
 
 // One CTA per window of packed tokens, head and side.  The tokens of a request that lie in one page are a group, handled by the CTA in whose window the
@@ -328,24 +333,26 @@ __device__ __forceinline__ void store_values(uint8_t* codes, const Block<C>& x, 
 }
 
 template <int C>
-__global__ void __maxnreg__(80) cache_append_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long ldk, long ldv, CachePages c, CacheStep s,
+__global__ void __maxnreg__(64) cache_append_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, long ldk, long ldv, CachePages c, CacheStep s,
                                                            int window) {
   __shared__ unsigned red[16];
   const int h = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5, D = c.D, P = 1 << c.shift;
   const bool values = blockIdx.z;
   const bf16* x = (values ? v : k) + h * D;
   const long ld = values ? ldv : ldk;
-  const int total = min(s.query_start[s.B], s.N), slabs = D / (32 * C);
+  const int slabs = D / (32 * C), all = s.query_start[s.B];
   int i = blockIdx.x * window;
-  const int end = min(i + window, total);
+  Request r = request_at(s, i);
+  const int total = min(all, s.N), end = min(i + window, total);
   while (i < end) {
-    const int b = request_at(s.query_start, s.B, i), first = s.query_start[b], next = s.query_start[b + 1];
-    const long pos = static_cast<long>(s.lengths[b]) - next + i;
-    const int off = static_cast<int>(pos & (P - 1)), m = max(min(min(next, total) - i, P - off), 1);
-    if (off != 0 && i != first) {                                      // of a group that began in another window
+    if (i >= r.next) r = request_at(s, i);
+    const long pos = static_cast<long>(r.length) - r.next + i;
+    const int off = static_cast<int>(pos & (P - 1)), m = max(min(min(r.next, total) - i, P - off), 1);
+    if (off != 0 && i != r.first) {                                    // of a group that began in another window
       i += m;
       continue;
     }
+    const int page = page_of(s, c, r.b, pos);                          // on its way beside the tokens
     // blocks of the group: 16 tokens each from off / 16 on, by columns
     const int g0 = off >> 4, blocks = (((off + m - 1) >> 4) - g0 + 1) * slabs;
     const bf16* src = x + static_cast<long>(i) * ld;
@@ -366,7 +373,6 @@ __global__ void __maxnreg__(80) cache_append_kernel(const bf16* __restrict__ k, 
       get(warp);
       top = max(top, amax_of(held));
     }
-    const int page = page_of(s, c, b, pos);
     const long ph = static_cast<long>(max(page, 0)) * c.H + h;
     const float before = c.scale[ph * 2 + values];
     top = __reduce_max_sync(0xffffffffu, top);
