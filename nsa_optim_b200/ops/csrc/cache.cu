@@ -214,6 +214,9 @@ __device__ __forceinline__ Request request_at(const CacheStep& s, int i) {
   return {lo + at, __shfl_sync(0xffffffffu, start, at), __shfl_sync(0xffffffffu, start, at + 1), __shfl_sync(0xffffffffu, length, at)};
 }
 
+// Quotient of numbers that are the same for all threads or nearly so: most often there is nothing to divide, or a power of two to divide by
+__device__ __forceinline__ int over(int y, int n) { return n == 1 ? y : (n & (n - 1)) == 0 ? y >> (31 - __clz(n)) : y / n; }
+
 // One CTA per window of packed tokens, head and side.  The tokens of a request that lie in one page are a group, handled by the CTA in whose window the
 // first of them lies: their largest magnitude gives the page's scale, codes that are there are rounded again where it grows, then the new ones are
 // stored.  A warp takes 16 tokens of 32 * C columns at a time, a lane C columns of them, so that it reads whole rows of 64 or 128 columns, its 16 tokens are
@@ -360,8 +363,8 @@ __global__ void __maxnreg__(64) cache_append_kernel(const bf16* __restrict__ k, 
     unsigned top = 0;
     auto full = [&](int t0) { return t0 >= off && t0 + 16 <= off + m; };
     auto get = [&](int y) {
-      const int t0 = (g0 + y / slabs) * 16;
-      const bf16* row = src + (t0 - off) * ld + (y % slabs) * 32 * C + lane * C;
+      const int yt = over(y, slabs), t0 = (g0 + yt) * 16;
+      const bf16* row = src + (t0 - off) * ld + (y - yt * slabs) * 32 * C + lane * C;
       if (full(t0)) load_block<C, true>(held, row, ld, t0, off, off + m);
       else load_block<C, false>(held, row, ld, t0, off, off + m);
     };
@@ -392,7 +395,7 @@ __global__ void __maxnreg__(64) cache_append_kernel(const bf16* __restrict__ k, 
     uint8_t* codes = (values ? c.v : c.k) + ph * P * D;
     for (int y = warp; y < blocks; y += warps) {
       if (y != warp) get(y);
-      const int d = (y % slabs) * 32 * C + lane * C, t0 = (g0 + y / slabs) * 16;
+      const int yt = over(y, slabs), d = (y - yt * slabs) * 32 * C + lane * C, t0 = (g0 + yt) * 16;
       if (full(t0) && !bad) store_full(codes, held, values, D, d, t0, inv);
       else if (values) store_values(codes, held, D, d, t0, off, off + m, ratio, inv, bad);
       else store_keys(codes, held, D, d, t0, off, off + m, ratio, inv, bad);
@@ -433,7 +436,7 @@ __global__ void __launch_bounds__(128) cache_values_kernel(CachePages c, const i
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int y = y0 + j * 128 * 8, token = y / (2 * D) * 2 + (y >> 6 & 1), d = (y % (2 * D) >> 7) * 64 + (y & 63);
+        const int y = y0 + j * 128 * 8, two = over(y, 2 * D), token = two * 2 + (y >> 6 & 1), d = (y - two * 2 * D >> 7) * 64 + (y & 63);
         if (y >= P * D) break;
         uint32_t o[4];
 #pragma unroll
@@ -449,7 +452,7 @@ __global__ void __launch_bounds__(128) cache_values_kernel(CachePages c, const i
   const uint8_t* codes = c.v + ph * P * D;
   const int slabs = D / (32 * C);
   for (int y = t >> 5; y < P / 16 * slabs; y += 4) {
-    const int t0 = y / slabs * 16, d = (y % slabs) * 32 * C + lane * C;
+    const int yt = over(y, slabs), t0 = yt * 16, d = (y - yt * slabs) * 32 * C + lane * C;
     uint32_t w[C][4];
 #pragma unroll
     for (int i = 0; i < C; ++i) {

@@ -317,16 +317,21 @@ __device__ __noinline__ void select(Smem& sm, const Part<T>& p, int b, int k) {
   const unsigned mine[kEach] = {four.x, four.y, four.z, four.w}, second[kEach] = {others.x, others.y, others.z, others.w};
   // the have-th largest of the pairs: the smallest of those with fewer than so many larger ones
   const unsigned g0 = max(four.x, four.y), g1 = max(four.z, four.w);
-  int before0 = 0, before1 = 0;
-  sm.pairs[lane] = make_uint2(g0, g1);
-  __syncwarp();
+  unsigned kth;
+  if (have == 1) {
+    kth = __reduce_max_sync(kAll, max(g0, g1));
+  } else {
+    int before0 = 0, before1 = 0;
+    sm.pairs[lane] = make_uint2(g0, g1);
+    __syncwarp();
 #pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const uint4 o = reinterpret_cast<const uint4*>(sm.pairs)[i];
-    before0 += (o.x > g0) + (o.y > g0) + (o.z > g0) + (o.w > g0);
-    before1 += (o.x > g1) + (o.y > g1) + (o.z > g1) + (o.w > g1);
+    for (int i = 0; i < 16; ++i) {
+      const uint4 o = reinterpret_cast<const uint4*>(sm.pairs)[i];
+      before0 += (o.x > g0) + (o.y > g0) + (o.z > g0) + (o.w > g0);
+      before1 += (o.x > g1) + (o.y > g1) + (o.z > g1) + (o.w > g1);
+    }
+    kth = __reduce_min_sync(kAll, min(before0 < have ? g0 : kAll, before1 < have ? g1 : kAll));
   }
-  const unsigned kth = __reduce_min_sync(kAll, min(before0 < have ? g0 : kAll, before1 < have ? g1 : kAll));
   int reach = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) reach += __popc(__ballot_sync(kAll, mine[i] >= kth));
