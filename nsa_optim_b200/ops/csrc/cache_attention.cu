@@ -17,6 +17,11 @@
 //  * Codes and their products are exact, and so is a query row scaled by a power of two to 2^13 .. 2^14 (bf16's 8 bits; what is 2^-28 of the row's
 //    largest value rounds).  Probabilities are rounded to 11 bits, relative to the row's largest product of probability and value scale: the value
 //    scale's exponent is added to x, and taken out again of the sum.  Sums are fp32.
+//
+// Measured, with the join: 8 contexts of 65 K tokens, 32 heads of 128 on 2: 55 us, 4.7 TB/s of codes; one token of each of 64 requests with 1 to 8192 tokens,
+// the same heads: 40 us, 3.4 TB/s, since a worker has 7 units, of which the first and the last few leave the memory idle (workers end between 24 and 32
+// us), and the join follows; eight drafted tokens of each of 32 requests with up to 12000 tokens, 32 heads on 8: 125 us, two tiles of 16 rows, 4600
+// cycles a unit of a worker (2700 for scores, 1800 for values), bounded by the latency of its products and exponentials: two workers per scheduler issue 44 % of the time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>

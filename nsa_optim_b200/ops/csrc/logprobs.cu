@@ -11,7 +11,12 @@
 // of the other pieces.  The k-th largest of the maxima of 64 pairs of threads is a bound that k logits reach, so only the four pieces of threads whose
 // maximum reaches it are read again (few more than k of 128 threads), and all pieces of a thread where a second four do.  A warp of its own does that,
 // and the row's end, while the others are in the next row.  What it waits for counts: behind 24 MB of copies a load takes 4 us, so that it reads what it
-// needs at once (when it read whole threads' pieces in turns, 4096 x 151936 logits with k = 8 took 413 us, with k = 1 230).
+// needs at once (when it read whole threads' pieces in turns, 4096 x 151936 logits with k = 8 took 413 us, with k = 1 230).  What it executes counts as well:
+// where each CTA has one row, nothing hides its end, and its instructions come from memory the first time (8 in about 50 cycles of a lone warp); where
+// it has many, they share the issue slots.  So loops stay loops, maxima are ranked by counting, and a single token's bound is one maximum.
+//
+// Measured: 4096 x 151936 bf16, k = 8: 235 us, 5.3 TB/s (backward 431 us, 5.8 TB/s); 8192 x 32000, k = 1: 116 us, 4.5 TB/s; 511 x 50257 fp32, k = 5: 28 us;
+// 64 x 151936, k = 20: 19 us, of which 5.5 to 7 until the last logit has been seen, 4.5 for the candidates, 2 for the slowest CTA of a cluster, 2 for places.
 //
 // Compiled without fast math: the logarithms at a row's end are the exact ones, the exponentials of its elements the hardware's.
 #include <cooperative_groups.h>
@@ -32,6 +37,8 @@ constexpr int kThreads = 128, kWarps = kThreads / 32;        // of the pass over
 constexpr int kCtas = 5;                  // per SM
 constexpr int kUnroll = 4, kHalves = 2;   // 16-byte pieces of a thread at a time; of a chunk
 constexpr int kChunk = kThreads * kUnroll * kHalves, kStages = 2;      // pieces that a bulk copy brings (16 KB); chunks on their way or in use
+// 4096 x 151936, k = 8, forward and backward 669 us, 8192 x 32000, k = 1 126 and 511 x 50257 27 when these were tried instead: four CTAs of three stages
+// 740 and 170; five of four stages of half a chunk 689, 124 and 29; six of three such stages 684, 121 and 31; halves in a loop 677, 122 and 29.
 constexpr int kTopMax = 32;               // tokens that the selection gives
 constexpr int kBuffer = 480;              // candidates for them
 constexpr int kParts = 8;                 // CTAs of a cluster

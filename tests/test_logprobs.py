@@ -196,6 +196,30 @@ def test_logits_that_are_not_finite(dev, dtype):
         assert dx[:3].isnan().all() and not dx[3].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("V,k", [(20011, 1), (20011, 20), (70001, 32)])
+def test_few_long_rows(dev, dtype, V, k):
+    """Rows that several blocks share: their likeliest tokens equal, in one part or spread over all, fewer than asked for, or not numbers."""
+    gen = torch.Generator().manual_seed(8)
+    x = logits(gen, 7, V, dtype, "cpu")
+    x[0] = -0.0
+    x[0, 3::7] = 0.0
+    x[1, V - 40:] = 20.0
+    x[2, ::V // 37] = 19.0
+    x[3] = -INF
+    x[4] = -INF
+    x[4, [5, V // 2, V - 1]] = torch.tensor([1.0, 3.0, 2.0]).to(dtype)
+    x[5, V // 3:] = torch.finfo(dtype).min
+    x[6, :] = torch.arange(V) / 1024
+    check(x.to(dev), tokens_of(gen, 7, V, dev), k, grads=grads_of(gen, 7, k, dev))
+    x = logits(gen, 2, V, dtype, "cpu")
+    x[0, [V - 2, 9]] = math.nan
+    x[1, V // 2] = INF
+    r = ops.token_logprobs(x.to(dev), torch.tensor([4, 4], device=dev), k)
+    assert r.logprob.isnan().all() and r.entropy.isnan().all() and r.top_index[0, 0] == 9 and r.top_index[1, 0] == V // 2
+    assert k == 1 or r.top_index[0, 1] == V - 2
+
+
 def test_tokens_that_do_not_count(dev):
     gen = torch.Generator().manual_seed(6)
     x = logits(gen, 5, 100, F32, dev)
