@@ -224,7 +224,7 @@ __device__ __forceinline__ int over(int y, int n) { return n == 1 ? y : (n & (n 
 // 256 tokens with more than 128 columns read the rest again).  The request, its length and the total come from one load each, side by side, and the page
 // number beside the tokens: what is left in a row is that, the tokens, a barrier and the codes.  34.7 K tokens of 8 heads of 128 columns: 50 us, 4.4 TB/s
 // of what it moves (142 MB read, 75 written), half of the issue slots (820 instructions for a warp's 64 codes a lane).  64 registers: twice as many warps as
-// 128 would allow are worth the 20 words that do not fit (both operators below together 88.6 us; with 48 101, 56 91.5, 80 92.2, 128 96.3).
+// 128 would allow are worth the 20 words that do not fit (with reading back, when that took 89, 48 101, 56 91.5, 80 92.2, 128 96.3).
 template <int C>
 struct Block {                             // 16 tokens, C columns of a lane
   uint32_t w[16][C / 2];
@@ -414,8 +414,9 @@ __global__ void __maxnreg__(64) cache_append_kernel(const bf16* __restrict__ k, 
 }
 
 // One CTA per page, head and side: bf16 values (n, P, H, D).  Keys 8 codes of a token at a time, four such loads before the first store; values 16 tokens of
-// C columns, so that a warp's stores are whole rows.  Bytes bound it: the same 34.7 K tokens 37 us, 5.3 TB/s (52 MB of the codes from memory, the rest from
-// L2, 144 MB written); in one CTA for both sides, keys by 16 and codes converted as whole numbers 39.
+// C columns, so that a warp's stores are whole rows.  Bytes bound it: the same 34.7 K tokens (52 MB of the codes from memory, the rest from L2, 144 MB written)
+// 37 us, 39 in one CTA for both sides with keys by 16 and codes converted as whole numbers.  Its results leave the caches first: appending and reading back
+// 89.5 -> 82.2 us.
 __device__ __forceinline__ float number_of(uint32_t w, int i, float s) {   // (code i of a word - 128) s, s a power of two: 2^23 + u by its bits
   return fmaf(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)), s, -8388736.f * s);
 }
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(128) cache_values_kernel(CachePages c, const i
           const uint32_t u = i < 2 ? w[j].x : w[j].y;
           o[i] = two_of(number_of(u, 2 * (i & 1), s), number_of(u, 2 * (i & 1) + 1, s));
         }
-        *reinterpret_cast<uint4*>(k + out + token * row + d) = make_uint4(o[0], o[1], o[2], o[3]);
+        __stcs(reinterpret_cast<uint4*>(k + out + token * row + d), make_uint4(o[0], o[1], o[2], o[3]));
       }
     }
     return;
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(128) cache_values_kernel(CachePages c, const i
     for (int tok = 0; tok < 16; ++tok) {
       bf16* to = v + out + (t0 + tok) * row + d;
       const uint32_t a = two_of(number_of(w[0][tok >> 2], tok & 3, s), number_of(w[1][tok >> 2], tok & 3, s));
-      if (C == 4) *reinterpret_cast<uint2*>(to) = make_uint2(a, two_of(number_of(w[C - 2][tok >> 2], tok & 3, s), number_of(w[C - 1][tok >> 2], tok & 3, s)));
+      if (C == 4) __stcs(reinterpret_cast<uint2*>(to), make_uint2(a, two_of(number_of(w[C - 2][tok >> 2], tok & 3, s), number_of(w[C - 1][tok >> 2], tok & 3, s))));
       else *reinterpret_cast<uint32_t*>(to) = a;
     }
   }

@@ -15,7 +15,7 @@
 // where each CTA has one row, nothing hides its end, and its instructions come from memory the first time (8 in about 50 cycles of a lone warp); where
 // it has many, they share the issue slots.  So loops stay loops, maxima are ranked by counting, and a single token's bound is one maximum.
 //
-// Measured: 4096 x 151936 bf16, k = 8: 235 us, 5.3 TB/s (backward 431 us, 5.8 TB/s); 8192 x 32000, k = 1: 116 us, 4.5 TB/s; 511 x 50257 fp32, k = 5: 28 us;
+// Measured: 4096 x 151936 bf16, k = 8: 235 us, 5.3 TB/s (backward 371 us, 6.7 TB/s, some of it from L2); 8192 x 32000, k = 1: 116 us, 4.5 TB/s; 511 x 50257 fp32, k = 5: 28 us;
 // 64 x 151936, k = 20: 19 us, of which 5.5 to 7 until the last logit has been seen, 4.5 for the candidates, 2 for the slowest CTA of a cluster, 2 for places.
 //
 // Compiled without fast math: the logarithms at a row's end are the exact ones, the exponentials of its elements the hardware's.
@@ -37,7 +37,7 @@ constexpr int kThreads = 128, kWarps = kThreads / 32;        // of the pass over
 constexpr int kCtas = 5;                  // per SM
 constexpr int kUnroll = 4, kHalves = 2;   // 16-byte pieces of a thread at a time; of a chunk
 constexpr int kChunk = kThreads * kUnroll * kHalves, kStages = 2;      // pieces that a bulk copy brings (16 KB); chunks on their way or in use
-// 4096 x 151936, k = 8, forward and backward 669 us, 8192 x 32000, k = 1 126 and 511 x 50257 27 when these were tried instead: four CTAs of three stages
+// 4096 x 151936, k = 8, forward and backward (an older one) 669 us, 8192 x 32000, k = 1 126 and 511 x 50257 27 when these were tried instead: four CTAs of three stages
 // 740 and 170; five of four stages of half a chunk 689, 124 and 29; six of three such stages 684, 121 and 31; halves in a loop 677, 122 and 29.
 constexpr int kTopMax = 32;               // tokens that the selection gives
 constexpr int kBuffer = 480;              // candidates for them
@@ -138,7 +138,7 @@ struct Vec<float> {
 template <class T>
 __device__ __forceinline__ Vec<T> load(const T* p) {                   // 16-byte aligned
   Vec<T> v;
-  *reinterpret_cast<uint4*>(&v.w) = __ldcs(reinterpret_cast<const uint4*>(p));
+  *reinterpret_cast<uint4*>(&v.w) = __ldg(reinterpret_cast<const uint4*>(p));
   return v;
 }
 
@@ -628,7 +628,10 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) logprobs_fwd_kernel(cons
 }
 
 // dx_j = -p_j (G + g_H (log p_j + H)), G the sum of the row's other gradients; theirs are added at their tokens.  One CTA per kBwdPieces pieces of a row.
-constexpr int kBwdThreads = 256, kBwdTurns = 4, kBwdPieces = kBwdThreads * kBwdTurns;
+// Bytes bound it, and how they are asked for: 4096 x 151936 bf16, forward and backward, with 8 loads of each of 128 threads 606 us, 8 of 96, 160, 192 and 256
+// 608, 610, 632 and 652, 4 of 256 667, 7 and 9 of 128 622, 16 of 64 772; loads that leave the caches first 618, stores that do not 617; rows from the
+// first on, not from the last, which the forward pass has left in L2, 608.
+constexpr int kBwdThreads = 128, kBwdTurns = 8, kBwdPieces = kBwdThreads * kBwdTurns;
 template <class T>
 __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const T* __restrict__ logits, long ld, const long long* __restrict__ tokens,
                                                                 const float2* __restrict__ stats, const float* __restrict__ entropy,
@@ -637,8 +640,8 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const T* __re
                                                                 T* __restrict__ dx_all, int V, int k, long long ignore, int chunks) {
   constexpr int kN = Vec<T>::kN;
   const int t = threadIdx.x;
-  const long row = blockIdx.x / chunks;
-  const int chunk = static_cast<int>(blockIdx.x - row * chunks);
+  const long row = (gridDim.x - 1 - blockIdx.x) / chunks;
+  const int chunk = static_cast<int>(gridDim.x - 1 - blockIdx.x - row * chunks);
   const T* x = logits + row * ld;
   T* dx = dx_all + row * V;
   // pieces where dx is 16-byte aligned; x is as well, or its elements are loaded one by one
