@@ -318,8 +318,8 @@ def cache_attention(q: Tensor, pages: KVPages, table: Tensor, query_start: Tenso
                     scale: Optional[float] = None, max_new: int = 1) -> Tensor:
     """Causal attention of packed queries (N, Hq, D), the last ``query_start[b + 1] - query_start[b]`` of each request's ``lengths[b]`` tokens, over the
     request's cached keys and values, their own among them (``window`` > 0: the last ``window`` of these alone).  Query heads share KV heads in equal
-    groups.  A query that sees nothing gets zeros.  ``max_new``, the most queries of a request, is a hint for the split of the
-    work: any value gives the same sums up to their order.  Inference only: no gradient is recorded."""
+    groups.  A query that sees nothing gets zeros, and so does a row of no request, before ``query_start[0]`` or from ``query_start[B]``
+    on.  ``max_new``, the most queries of a request, is a hint for the split of the work: any value gives the same sums up to their order.  Inference only: no gradient is recorded."""
     if _use_native(q, "cache"):
         return native_module().cache_attention(q, pages, table, query_start, lengths, window, scale, max_new)
     return cache.attention(q.detach(), pages, table, query_start, lengths, window, scale)

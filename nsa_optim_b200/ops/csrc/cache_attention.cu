@@ -49,6 +49,7 @@ struct AttnParams {
   float2* part_ml;      // (CTA, 2, rows)
   struct Join* join;    // (CTA)
   int Hq, G, window;
+  int ends;             // 1: the first request of the call is among these, 2: the last one
   unsigned long long per_g;   // ceil(2^32 / G): row / G of rows below 2^32 / G is a multiplication
   float scale;          // times log2(e)
   KernelStatus* status;
@@ -914,14 +915,24 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
   }
 }
 
-// Parts of items that several CTAs worked on: CTA (c, part) takes some rows of the item that begins in CTA c of the kernel before.
+// Parts of items that several CTAs worked on: CTA (c, part) takes some rows of the item that begins in CTA c of the kernel before.  Rows of no request, before
+// the first one's and behind the last one's, are in no item: all CTAs together set them to zero.
 constexpr int kJoinParts = 4;
+__device__ __forceinline__ void clear_rows(const AttnParams& p, long from, long to, long width) {      // width: 16-byte pieces of a row
+  uint4* out = reinterpret_cast<uint4*>(p.o);
+  const long step = static_cast<long>(gridDim.x) * kJoinParts * 128;
+  for (long i = from * width + (static_cast<long>(blockIdx.x) * kJoinParts + blockIdx.y) * 128 + threadIdx.x; i < to * width; i += step)
+    out[i] = make_uint4(0, 0, 0, 0);
+}
 template <int D, int R>
 __global__ void __launch_bounds__(128) cache_attn_join_kernel(const __grid_constant__ AttnParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x;
   const Join j = p.join[c];
+  const int first = p.ends & 1 ? p.s.query_start[0] : 0, behind = p.ends & 2 ? p.s.query_start[p.s.B] : p.s.N;
+  clear_rows(p, 0, min(first, p.s.N), static_cast<long>(p.Hq) * D / 8);
+  clear_rows(p, max(behind, 0), p.s.N, static_cast<long>(p.Hq) * D / 8);
   if (!j.any) return;
   const int last = static_cast<int>((j.end - 1) / j.each / kWarps);
   for (int e = blockIdx.y * 128 + threadIdx.x; e < R * (D / 4); e += kJoinParts * 128) {
@@ -1037,6 +1048,7 @@ extern "C" int nsa_cache_attention(const void* q, long ldq, const void* kc, cons
   cudaError_t e = cudaSuccess;
   for (int b = 0; b < B && e == cudaSuccess; b += kMaxRequests) {      // a launch for each 768 requests, on the same scratch
     p.s = CacheStep{table + static_cast<long>(b) * W, query_start + b, lengths + b, B - b < kMaxRequests ? B - b : kMaxRequests, W, N};
+    p.ends = (b == 0 ? 1 : 0) | (b + kMaxRequests >= B ? 2 : 0);
     if (D == 128)
       e = rows == 8 ? run<128, 8>(p, grid, st) : run<128, 16>(p, grid, st);
     else

@@ -548,3 +548,44 @@ def test_tensors_on_two_devices_are_refused(native):
         ops.cache_append(ops.KVPages(*(t.cpu() for t in g["p"])), g["k"], g["v"], g["table"], g["start"], g["lengths"])
     with pytest.raises(ValueError):
         ops.cache_plan(g["lengths"], g["new"].cpu(), g["table"], g["free"], g["count"], 3, 16)
+
+
+# ------------------------------------------------------------------------------------------------ rows of no request
+def poisoned(like):
+    """Leaves NaN in the memory that the allocator hands out next."""
+    if like.is_cuda:
+        for _ in range(2):
+            some = [torch.full_like(like, math.nan) for _ in range(16)]
+            del some
+
+
+@pytest.mark.parametrize("Hq,D", [(4, 64), (16, 128), (2, 192)])
+@pytest.mark.parametrize("start", [[0, 2, 3], [5, 7, 10], [3, 3, 3]])
+def test_queries_of_no_request_get_zeros(dev, Hq, D, start):
+    """More places than tokens, as in a step of a fixed size, and requests out of the middle of a packed step."""
+    gen = torch.Generator().manual_seed(14)
+    lengths = [40, 70]
+    c, table = filled(dev, gen, lengths, 1, D, 16)
+    q = some(gen, 12, Hq, D, dev)
+    args = (c.t, i32(table, dev), i32(start, dev), i32(lengths, dev))
+    poisoned(q)
+    got = ops.cache_attention(q, *args)
+    close(got, *attention_oracle(q, c, table, start, lengths, 0, D ** -0.5))
+    assert not got[:start[0]].any() and not got[start[2]:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [768, 769, 1600])
+def test_requests_of_several_launches(native, B):
+    """More requests than one launch takes, of one to three new tokens or none, with places of nobody before and behind them."""
+    gen = torch.Generator().manual_seed(B)
+    new = torch.randint(0, 4, (B,), generator=gen).tolist()
+    lengths = [n + p for n, p in zip(new, torch.randint(0, 60, (B,), generator=gen).tolist())]
+    c, table = filled("cuda", gen, [max(n, 1) for n in lengths], 1, 64, 16)
+    start = [3 + sum(new[:i]) for i in range(B + 1)]
+    q = some(gen, start[-1] + 4, 2, 64, "cuda")
+    args = (c.t, i32(table, "cuda"), i32(start, "cuda"), i32(lengths, "cuda"))
+    poisoned(q)
+    got = ops.cache_attention(q, *args, max_new=3)
+    close(got, *attention_oracle(q, c, table, start, lengths, 0, 0.125))
+    assert not got[:3].any() and not got[start[-1]:].any()
