@@ -300,7 +300,7 @@ def cache_release(finished: Tensor, lengths: Tensor, table: Tensor, free: Tensor
 def cache_append(pages: KVPages, k: Tensor, v: Tensor, table: Tensor, query_start: Tensor, lengths: Tensor) -> None:
     """Rounds the keys and values (N, Hkv, D) of a step's packed tokens to 8 bits and stores them, in place, as the last
     ``query_start[b + 1] - query_start[b]`` of each request's ``lengths[b]`` tokens.  A page's first token sets its scale anew; larger values raise it later,
-    and the page's codes with it.  Tokens without a page are left out."""
+    and the page's codes with it.  Tokens without a page are left out, and so are rows of no request (before ``query_start[0]`` or from ``query_start[B]`` on)."""
     if _use_native(k, "cache"):
         return native_module().cache_append(pages, k, v, table, query_start, lengths)
     return cache.append(pages, k, v, table, query_start, lengths)

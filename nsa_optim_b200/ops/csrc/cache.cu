@@ -352,6 +352,10 @@ __global__ void __maxnreg__(64) cache_append_kernel(const bf16* __restrict__ k, 
   const int total = min(all, s.N), end = min(i + window, total);
   while (i < end) {
     if (i >= r.next) r = request_at(s, i);
+    if (i < r.first) {                                                 // of no request: the first one begins behind it
+      i = r.first;
+      continue;
+    }
     const long pos = static_cast<long>(r.length) - r.next + i;
     const int off = static_cast<int>(pos & (P - 1)), m = max(min(min(r.next, total) - i, P - off), 1);
     if (off != 0 && i != r.first) {                                    // of a group that began in another window

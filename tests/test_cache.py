@@ -589,3 +589,19 @@ def test_requests_of_several_launches(native, B):
     got = ops.cache_attention(q, *args, max_new=3)
     close(got, *attention_oracle(q, c, table, start, lengths, 0, 0.125))
     assert not got[:3].any() and not got[start[-1]:].any()
+
+
+@pytest.mark.parametrize("before", [1, 5, 40, 2100])
+def test_tokens_of_no_request_are_left_out(dev, before):
+    """Requests out of the middle of a packed step: rows before the first one's and behind the last one's are not theirs."""
+    gen = torch.Generator().manual_seed(before)
+    past, new, P = [40, 0, 20], [3, 0, 40], 16
+    total = [a + b for a, b in zip(past, new)]
+    table, _ = make_tables(total, 5, P, gen, 0)
+    c = Cache(dev, 1 + max(max(r) for r in table), 2, 64, P)
+    at = [0, 40, 40, 60]
+    c.append(some(gen, 60, 2, 64, dev), some(gen, 60, 2, 64, dev), table, at, past)
+    start = [before, before + 3, before + 3, before + 43]
+    rows = start[-1] + 7
+    c.append(some(gen, rows, 2, 64, dev, size=2.0), some(gen, rows, 2, 64, dev, size=0.5), table, start, total)
+    c.check()
