@@ -16,7 +16,7 @@
 //    32 contexts of up to 12000 tokens took 268 us, then 240.)
 //  * Codes and their products are exact, and so is a query row scaled by a power of two to 2^13 .. 2^14 (bf16's 8 bits; what is 2^-28 of the row's
 //    largest value rounds).  Probabilities are rounded to 11 bits, relative to the row's largest product of probability and value scale: the value
-//    scale's exponent is added to x, and taken out again of the sum.  Sums are fp32.
+//    scale's exponent is added to x, and taken out again of the sum.  Sums are fp32.  Scores may be of any size up to 2^119.
 //
 // Measured, with the join: 8 contexts of 65 K tokens, 32 heads of 128 on 2: 55 us, 4.7 TB/s of codes; one token of each of 64 requests with 1 to 8192 tokens,
 // the same heads: 40 us, 3.4 TB/s, since a worker has 7 units, of which the first and the last few leave the memory idle (workers end between 24 and 32
@@ -284,6 +284,9 @@ struct Query {
 
 // Scores s of two rows and some keys of a lane become probabilities.  get(row, n) is the reference to its n-th score, key(n) that one's token in the
 // lane's sub-block, N of them; reduce() the maximum over the lanes that share the rows, rescale(f) multiplies their outputs.
+// Where x or c is so large that m, b and x may round apart by a part of 1, scores are taken relative to the lane's largest first, so that no x is above 0; what
+// fp32 then loses, it loses of scores that are as far apart.
+constexpr float kFar = 0x1p19f;
 struct Running {
   float factor[2], off[2];   // of the lane's two rows
   int pos[2];                // their positions; -1: no row
@@ -320,22 +323,32 @@ __device__ __forceinline__ void references(Running& w, Get get, Key key, Reduce 
     top[0] = fmaxf(top[0], get(0, n));
     top[1] = fmaxf(top[1], get(1, n));
   }
-  bool moved = false;
+  float m[2];
+  bool moved = false, far = false;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float m = fmaxf(w.m[i], reduce(fmaf(top[i], a[i], c[i])));
-    moved |= m != w.m[i];
-    ref[i] = m == -CUDART_INF_F ? 0.f : m;
-    top[i] = m;
+    m[i] = fmaxf(w.m[i], reduce(fmaf(top[i], a[i], c[i])));
+    moved |= m[i] != w.m[i];
+    ref[i] = m[i] == -CUDART_INF_F ? 0.f : m[i];
+    far |= fmaxf(fabsf(ref[i]), fabsf(c[i])) > kFar;
     b[i] = c[i] - ref[i];
   }
-  if (__any_sync(0xffffffffu, moved)) {
+  if (__any_sync(0xffffffffu, moved || far)) {
     const float2 f = make_float2(ex2(w.m[0] - ref[0]), ex2(w.m[1] - ref[1]));
-    w.m[0] = top[0];
-    w.m[1] = top[1];
+    w.m[0] = m[0];
+    w.m[1] = m[1];
     w.l[0] *= f.x;
     w.l[1] *= f.y;
     rescale(f);
+    if (far) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (top[i] == -CUDART_INF_F) continue;
+        b[i] = fmaf(top[i], a[i], c[i]) - ref[i];
+#pragma unroll
+        for (int n = 0; n < N; ++n) get(i, n) -= top[i];
+      }
+    }
   }
   out = ex2(-ev);
 }

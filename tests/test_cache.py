@@ -605,3 +605,30 @@ def test_tokens_of_no_request_are_left_out(dev, before):
     rows = start[-1] + 7
     c.append(some(gen, rows, 2, 64, dev, size=2.0), some(gen, rows, 2, 64, dev, size=0.5), table, start, total)
     c.check()
+
+
+# ------------------------------------------------------------------------------------------------ probabilities and scores of any size
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e7, 1e8, 1e9, 1e20, 1e30])
+@pytest.mark.parametrize("sign", [1, -1, 0])
+def test_scores_far_from_zero(dev, size, sign):
+    """Finite scores of any size, all positive, all negative or both.  Queries are drawn until the largest score stands out by more than fp32 can lose: it takes
+    all of the probability."""
+    gen = torch.Generator().manual_seed(15)
+    lengths, D, P = [90, 33, 5], 64, 16
+    table, _ = make_tables(lengths, 6, P, gen, 0)
+    c = Cache(dev, 1 + max(max(r) for r in table), 1, D, P)
+    k, v = some(gen, 128, 1, D, dev), some(gen, 128, 1, D, dev)
+    c.append(k.abs() if sign else k, v, table, [0, 90, 123, 128], lengths)
+    q = torch.empty(5, 4, D, dtype=BF)
+    for i, (b, keys) in enumerate(((0, 90), (1, 31), (1, 32), (1, 33), (2, 5))):
+        pages = torch.tensor([table[b][j // P] for j in range(keys)])
+        seen = c.values()[0][pages, torch.arange(keys) % P, 0]
+        for h in range(4):
+            stands_out = False
+            while not stands_out:
+                q[i, h] = (torch.randn(D, generator=gen).abs() * sign if sign else torch.randn(D, generator=gen)) * size
+                x = seen @ q[i, h].double()
+                gap = -x.topk(2).values.diff().item()
+                stands_out = gap > x.abs().max() * 2.0 ** -10 and gap / 8 > 50
+    for most in (1, 3):
+        attend(c, q.to(dev), table, [1, 3, 1], lengths, max_new=most)
