@@ -16,7 +16,8 @@
 //    32 contexts of up to 12000 tokens took 268 us, then 240.)
 //  * Codes and their products are exact, and so is a query row scaled by a power of two to 2^13 .. 2^14 (bf16's 8 bits; what is 2^-28 of the row's
 //    largest value rounds).  Probabilities are rounded to 11 bits, relative to the row's largest product of probability and value scale: the value
-//    scale's exponent is added to x, and taken out again of the sum.  Sums are fp32.  Scores may be of any size up to 2^119.
+//    scale's exponent is added to x, and taken out again of the sum.  Of products below 2^-29 of the largest fewer bits are kept, none below 2^-40.  Sums
+//    are fp32.  Scores may be of any size up to 2^119.
 //
 // Measured, with the join: 8 contexts of 65 K tokens, 32 heads of 128 on 2: 55 us, 4.7 TB/s of codes; one token of each of 64 requests with 1 to 8192 tokens,
 // the same heads: 40 us, 3.4 TB/s, since a worker has 7 units, of which the first and the last few leave the memory idle (workers end between 24 and 32
@@ -287,6 +288,8 @@ struct Query {
 // Where x or c is so large that m, b and x may round apart by a part of 1, scores are taken relative to the lane's largest first, so that no x is above 0; what
 // fp32 then loses, it loses of scores that are as far apart.
 constexpr float kFar = 0x1p19f;
+// The largest probability is held as 2^15, near the end of f16's range: others have 11 bits down to 2^-29 of it.  Outputs and sums share the factor.
+constexpr float kUp = 15.f;
 struct Running {
   float factor[2], off[2];   // of the lane's two rows
   int pos[2];                // their positions; -1: no row
@@ -331,7 +334,7 @@ __device__ __forceinline__ void references(Running& w, Get get, Key key, Reduce 
     moved |= m[i] != w.m[i];
     ref[i] = m[i] == -CUDART_INF_F ? 0.f : m[i];
     far |= fmaxf(fabsf(ref[i]), fabsf(c[i])) > kFar;
-    b[i] = c[i] - ref[i];
+    b[i] = c[i] - ref[i] + kUp;
   }
   if (__any_sync(0xffffffffu, moved || far)) {
     const float2 f = make_float2(ex2(w.m[0] - ref[0]), ex2(w.m[1] - ref[1]));
@@ -344,7 +347,7 @@ __device__ __forceinline__ void references(Running& w, Get get, Key key, Reduce 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (top[i] == -CUDART_INF_F) continue;
-        b[i] = fmaf(top[i], a[i], c[i]) - ref[i];
+        b[i] = fmaf(top[i], a[i], c[i]) - ref[i] + kUp;
 #pragma unroll
         for (int n = 0; n < N; ++n) get(i, n) -= top[i];
       }

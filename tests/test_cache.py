@@ -632,3 +632,23 @@ def test_scores_far_from_zero(dev, size, sign):
                 stands_out = gap > x.abs().max() * 2.0 ** -10 and gap / 8 > 50
     for most in (1, 3):
         attend(c, q.to(dev), table, [1, 3, 1], lengths, max_new=most)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq", [8, 16])
+def test_a_token_that_takes_nearly_all(native, Hq):
+    """65536 keys; the first takes 99.7 % of the probability and has the value 0, so that the output is the sum of what is left, 2^-24 of the largest each.  As many
+    row tiles as the kernel has workers (8 per SM), so that one of them walks a whole context.  The other values are all 1: errors are relative, 2^-8
+    of the result's rounding, 2^-11 of the probabilities', as much again for sums and exponentials."""
+    P, D, L = 64, 64, 65536
+    n = 8 * torch.cuda.get_device_properties(0).multi_processor_count
+    k, v = torch.zeros(L, 1, D, dtype=BF, device="cuda"), torch.ones(L, 1, D, dtype=BF, device="cuda")
+    k[0, 0, 0], v[0] = 8.0, 0.0
+    t, table = ops.cache_pages(L // P, 1, D, P, device="cuda"), torch.arange(L // P, dtype=torch.int32, device="cuda")[None]
+    ops.cache_append(t, k, v, table, i32([0, L], "cuda"), i32([L], "cuda"))
+    q = torch.zeros(n, Hq, D, dtype=BF, device="cuda")
+    q[:, :, 0] = 16.875                                                # e^16.875 with the first key, 1 with the others
+    got = ops.cache_attention(q, t, table, i32([0, n], "cuda"), i32([L], "cuda")).double().cpu()
+    others = torch.arange(L - n, L, dtype=torch.double)
+    want = (others / (others + math.exp(16.875)))[:, None, None]
+    assert ((got - want).abs() <= want * (2.0 ** -8 + 2.0 ** -10)).all(), (got[0, 0, 0], want[0], got[-1, -1, -1], want[-1])
