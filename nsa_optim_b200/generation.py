@@ -44,9 +44,13 @@ class PagedCache:
         self.held = [0] * requests                           # the lengths as the host knows them
 
     def step(self, new: Sequence[int]) -> "CacheStep":
-        """Makes room for ``new[b]`` tokens of each request; the result goes to the model as ``past_key_values``."""
+        """Makes room for ``new[b]`` tokens of each request; the result goes to the model as ``past_key_values``.  A step for which there are too few
+        pages is refused and changes nothing."""
         if len(new) != self.requests or min(new) < 0:
             raise ValueError(f"a count of new tokens for each of {self.requests} requests is needed")
+        need, pages = sum(-(-(a + b) // self.page_size) for a, b in zip(self.held, new)), self.free.numel()
+        if need > pages:
+            raise ValueError(f"the step needs {need} pages of {self.page_size} tokens, the cache has {pages}")
         counts = torch.tensor(list(new), dtype=torch.int32).to(self.lengths.device, non_blocking=True)
         plan = ops.cache_plan(self.lengths, counts, self.table, self.free, self.free_count, sum(new), self.page_size)
         self.lengths, self.free_count = plan.lengths, plan.free_count

@@ -192,3 +192,32 @@ def test_a_step_is_native(native):
         finally:
             torch.cuda.set_sync_debug_mode("default")
         assert native.fallback_counts() == {}
+
+
+def state_of(cache):
+    return cache.held, cache.lengths.tolist(), int(cache.free_count), sorted(cache.free.tolist()), cache.table.tolist()
+
+
+def test_a_step_beyond_the_cache_is_refused(dev):
+    """A step that needs more pages than there are changes nothing; one that needs them all goes through."""
+    model = small(dev, layers=1)
+    cache = PagedCache(model, requests=3, tokens=32, page_size=16)            # five pages
+    cache.step([17, 0, 16])
+    before = state_of(cache)
+    for new in ([0, 33, 0], [16, 0, 17], [0, 1, 17], [49, 0, 0]):
+        with pytest.raises(ValueError):
+            cache.step(new)
+        assert state_of(cache) == before
+    assert int(cache.step([15, 1, 16]).plan.shortfall) == 0 and int(cache.free_count) == 0
+    cache.release([False, True, False])
+    cache.step([1, 0, 0])
+    assert int(cache.free_count) == 0
+
+
+def test_a_cache_too_small_for_the_prompts_is_refused(dev):
+    model = small(dev)
+    prompts = texts([60, 55])
+    with pytest.raises(ValueError):
+        generate(model, prompts, 8, cache=PagedCache(model, requests=2, tokens=48, page_size=16))
+    cache = PagedCache(model, requests=2, tokens=112, page_size=16)            # nine pages: 63 and 60 tokens are eight
+    assert generate(model, prompts, 8, cache=cache).tokens == generate(model, prompts, 8).tokens
