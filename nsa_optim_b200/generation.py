@@ -121,32 +121,36 @@ def generate(model: TransformerModel, prompts: Sequence[Sequence[int]], max_new_
         cache = PagedCache(model, B, sum(len(p) + max_new_tokens for p in prompts))
     if cache.requests < B:
         raise ValueError(f"the cache holds {cache.requests} requests, {B} were given")
+    if any(cache.held[:B]):
+        raise ValueError(f"the cache's first {B} requests have to be empty: they hold {cache.held[:B]} tokens")
     rows = list(range(B))                                    # requests that go on
     new = [len(p) for p in prompts] + [0] * (cache.requests - B)
     tokens = torch.tensor([t for p in prompts for t in p], device=device)
     chosen, kept = [], []
     none = torch.full((cache.requests,), -1, dtype=torch.long, device=device)
-    for n in range(max_new_tokens):
-        step = cache.step(new)
-        h = model(tokens.unsqueeze(0), past_key_values=step, return_hidden=True)[0]
-        r = ops.token_logprobs(ops.linear(h[0, step.last_rows()], model.output_weight()), none, top_k)
-        if temperature > 0 and top_k > 1:
-            pick = torch.multinomial(torch.softmax(r.top_logprob / temperature, -1), 1, generator=generator)
-        else:
-            pick = torch.zeros(cache.requests, 1, dtype=torch.long, device=device)
-        tok, lp = r.top_index.gather(1, pick)[:, 0], r.top_logprob.gather(1, pick)[:, 0]
-        chosen.append((tok, lp, r.entropy))
-        kept.append((rows, r.top_index, r.top_logprob))
-        if end_token is not None:
-            ended = (tok == end_token).tolist()              # the one thing that the host waits for
-            cache.release([b in rows and ended[b] for b in range(cache.requests)])
-            rows = [b for b in rows if not ended[b]]
-            if not rows:
-                break
-        new = [1 if b in rows else 0 for b in range(cache.requests)]
-        tokens = tok[rows] if len(rows) < cache.requests else tok
-    if rows:
-        cache.release([b in rows for b in range(cache.requests)])
+    try:
+        for n in range(max_new_tokens):
+            step = cache.step(new)
+            h = model(tokens.unsqueeze(0), past_key_values=step, return_hidden=True)[0]
+            r = ops.token_logprobs(ops.linear(h[0, step.last_rows()], model.output_weight()), none, top_k)
+            if temperature > 0 and top_k > 1:
+                pick = torch.multinomial(torch.softmax(r.top_logprob / temperature, -1), 1, generator=generator)
+            else:
+                pick = torch.zeros(cache.requests, 1, dtype=torch.long, device=device)
+            tok, lp = r.top_index.gather(1, pick)[:, 0], r.top_logprob.gather(1, pick)[:, 0]
+            chosen.append((tok, lp, r.entropy))
+            kept.append((rows, r.top_index, r.top_logprob))
+            if end_token is not None:
+                ended = (tok == end_token).tolist()          # the one thing that the host waits for
+                cache.release([b in rows and ended[b] for b in range(cache.requests)])
+                rows = [b for b in rows if not ended[b]]
+                if not rows:
+                    break
+            new = [1 if b in rows else 0 for b in range(cache.requests)]
+            tokens = tok[rows] if len(rows) < cache.requests else tok
+    finally:                                                 # also where a step was refused or interrupted
+        if rows:
+            cache.release([b in rows for b in range(cache.requests)])
     out = Generated([[] for _ in range(B)], [[] for _ in range(B)], [[] for _ in range(B)], [[] for _ in range(B)] if alternatives else None)
     for (tok, lp, h), (alive, index, top) in zip(chosen, kept):
         tok, lp, h = tok.tolist(), lp.tolist(), h.tolist()

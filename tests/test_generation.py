@@ -221,3 +221,40 @@ def test_a_cache_too_small_for_the_prompts_is_refused(dev):
         generate(model, prompts, 8, cache=PagedCache(model, requests=2, tokens=48, page_size=16))
     cache = PagedCache(model, requests=2, tokens=112, page_size=16)            # nine pages: 63 and 60 tokens are eight
     assert generate(model, prompts, 8, cache=cache).tokens == generate(model, prompts, 8).tokens
+
+
+def test_a_cache_in_use_is_refused(dev):
+    """generate takes the first requests of a cache: they have to be empty, others may be under way."""
+    model = small(dev)
+    prompts = texts([21, 9])
+    want = generate(model, prompts, 5).tokens
+    cache = PagedCache(model, requests=3, tokens=200, page_size=16)
+    cache.step([0, 0, 20])
+    assert generate(model, prompts, 5, cache=cache).tokens == want and cache.held == [0, 0, 20]
+    cache.step([0, 3, 0])
+    before = state_of(cache)
+    with pytest.raises(ValueError):
+        generate(model, prompts, 5, cache=cache)
+    assert state_of(cache) == before
+
+
+@pytest.mark.parametrize("call", [1, 4])
+def test_an_interrupted_generation_leaves_its_cache_empty(dev, call, monkeypatch):
+    model = small(dev)
+    prompts = texts([21, 9])
+    cache = PagedCache(model, requests=3, tokens=200, page_size=16)
+    cache.step([0, 0, 20])
+    want = generate(model, prompts, 6, cache=cache).tokens
+    real, calls = ops.token_logprobs, []
+
+    def interrupted(*args):
+        calls.append(1)
+        if len(calls) == call:
+            raise KeyboardInterrupt
+        return real(*args)
+    monkeypatch.setattr(ops, "token_logprobs", interrupted)
+    with pytest.raises(KeyboardInterrupt):
+        generate(model, prompts, 6, cache=cache)
+    monkeypatch.undo()
+    assert cache.held == cache.lengths.tolist() == [0, 0, 20] and int(cache.free_count) == cache.free.numel() - 2
+    assert generate(model, prompts, 6, cache=cache).tokens == want
