@@ -127,7 +127,7 @@ def generate(model: TransformerModel, prompts: Sequence[Sequence[int]], max_new_
     new = [len(p) for p in prompts] + [0] * (cache.requests - B)
     tokens = torch.tensor([t for p in prompts for t in p], device=device)
     chosen, kept = [], []
-    none = torch.full((cache.requests,), -1, dtype=torch.long, device=device)
+    none = torch.full((cache.requests,), -100, dtype=torch.long, device=device)
     try:
         for n in range(max_new_tokens):
             step = cache.step(new)

@@ -258,3 +258,16 @@ def test_an_interrupted_generation_leaves_its_cache_empty(dev, call, monkeypatch
     monkeypatch.undo()
     assert cache.held == cache.lengths.tolist() == [0, 0, 20] and int(cache.free_count) == cache.free.numel() - 2
     assert generate(model, prompts, 6, cache=cache).tokens == want
+
+
+def test_rows_without_a_given_token_are_ignored_ones(dev, monkeypatch):
+    """A debug build records tokens that are neither ignored nor in the vocabulary."""
+    model = small(dev, layers=1)
+    real, given = ops.token_logprobs, []
+
+    def watched(logits, tokens, top_k=0, ignore_index=-100):
+        given.append((tokens.tolist(), ignore_index))
+        return real(logits, tokens, top_k, ignore_index)
+    monkeypatch.setattr(ops, "token_logprobs", watched)
+    generate(model, texts([3, 5]), 3)
+    assert len(given) == 3 and all(t == ignored for tokens, ignored in given for t in tokens)
