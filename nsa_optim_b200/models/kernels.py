@@ -117,9 +117,11 @@ class RotaryEmbedding(nn.Module):
         self.max_seq_len_cached = seq_len
 
     def rows(self, positions: Tensor, limit: int) -> Tuple[Tensor, Tensor]:
-        """The rows of positions below ``limit``, a number that the host knows, so that it does not wait for their maximum."""
-        if limit > self.max_seq_len_cached or self.cos_cached.device != positions.device:
-            self._set_cos_sin_cache(max(limit, self._initial), device=positions.device)
+        """The rows of positions below ``limit``, a number that the host knows, so that it does not wait for their maximum.  The tables at least double
+        when they grow: ``limit`` rises by one a generated token."""
+        have = self.max_seq_len_cached
+        if limit > have or self.cos_cached.device != positions.device:
+            self._set_cos_sin_cache(max(limit, 2 * have if limit > have else have, self._initial), device=positions.device)
         return self.cos_cached[positions], self.sin_cached[positions]
 
     def forward(self, x: Tensor, position_ids: Optional[Tensor] = None, seq_len: Optional[int] = None

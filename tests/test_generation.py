@@ -271,3 +271,16 @@ def test_rows_without_a_given_token_are_ignored_ones(dev, monkeypatch):
     monkeypatch.setattr(ops, "token_logprobs", watched)
     generate(model, texts([3, 5]), 3)
     assert len(given) == 3 and all(t == ignored for tokens, ignored in given for t in tokens)
+
+
+def test_rotary_tables_grow_seldom(dev, monkeypatch):
+    """Requests beyond the configured length: the table doubles instead of being built again for every token, and keeps its values."""
+    from nsa_optim_b200.models.kernels import RotaryEmbedding
+    emb, built = RotaryEmbedding(64, 16), []
+    real = RotaryEmbedding._set_cos_sin_cache
+    monkeypatch.setattr(RotaryEmbedding, "_set_cos_sin_cache", lambda self, n, device=None: (built.append(n), real(self, n, device=device)))
+    want = ops.oracle.rope_tables(64, 300, emb.base, device=dev)
+    for n in list(range(1, 65)) + [300]:
+        cos, sin = emb.rows(torch.arange(n, device=dev), n)
+        assert torch.equal(cos, want[0][:n]) and torch.equal(sin, want[1][:n])
+    assert len(built) <= 4 and max(built) <= 600
