@@ -123,9 +123,14 @@ def generate(model: TransformerModel, prompts: Sequence[Sequence[int]], max_new_
         raise ValueError(f"the cache holds {cache.requests} requests, {B} were given")
     if any(cache.held[:B]):
         raise ValueError(f"the cache's first {B} requests have to be empty: they hold {cache.held[:B]} tokens")
+
+    def there(numbers):                                      # a list on the device, without waiting for it
+        return torch.tensor(numbers).to(device, non_blocking=True)
+
     rows = list(range(B))                                    # requests that go on
+    live = there(rows)
     new = [len(p) for p in prompts] + [0] * (cache.requests - B)
-    tokens = torch.tensor([t for p in prompts for t in p], device=device)
+    tokens = there([t for p in prompts for t in p])
     chosen, kept = [], []
     none = torch.full((cache.requests,), -100, dtype=torch.long, device=device)
     try:
@@ -146,8 +151,9 @@ def generate(model: TransformerModel, prompts: Sequence[Sequence[int]], max_new_
                 rows = [b for b in rows if not ended[b]]
                 if not rows:
                     break
+                live = there(rows)
             new = [1 if b in rows else 0 for b in range(cache.requests)]
-            tokens = tok[rows] if len(rows) < cache.requests else tok
+            tokens = tok[live] if len(rows) < cache.requests else tok
     finally:                                                 # also where a step was refused or interrupted
         if rows:
             cache.release([b in rows for b in range(cache.requests)])

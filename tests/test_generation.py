@@ -284,3 +284,28 @@ def test_rotary_tables_grow_seldom(dev, monkeypatch):
         cos, sin = emb.rows(torch.arange(n, device=dev), n)
         assert torch.equal(cos, want[0][:n]) and torch.equal(sin, want[1][:n])
     assert len(built) <= 4 and max(built) <= 600
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sampled", [False, True])
+def test_generation_does_not_wait(native, sampled, monkeypatch):
+    """Without an end token nothing makes the host wait before the results are read, also in a cache with more requests than prompts."""
+    model = small("cuda")
+    cache = PagedCache(model, requests=5, tokens=300)
+    prompts = texts([30, 7, 50])
+    kw = dict(cache=cache, temperature=0.8, top_k=4) if sampled else dict(cache=cache)
+    generate(model, prompts, 4, **kw)
+    real, read = PagedCache.release, []
+
+    def release(self, finished):                                # the last thing before results are read
+        real(self, finished)
+        read.append(1)
+        torch.cuda.set_sync_debug_mode("default")
+    monkeypatch.setattr(PagedCache, "release", release)
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        generate(model, prompts, 4, **kw)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert len(read) == 1
