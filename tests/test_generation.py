@@ -309,3 +309,26 @@ def test_generation_does_not_wait(native, sampled, monkeypatch):
     finally:
         torch.cuda.set_sync_debug_mode("default")
     assert len(read) == 1
+
+
+def test_requests_go_on_when_others_end(dev):
+    """What is generated behind another request's end: the same tokens as without an end, up to the request's own, exactly on the CPU, on a GPU up to a near tie (products
+    of other shapes round differently)."""
+    model = small(dev)
+    prompts = texts([21, 64, 7, 30])
+    cache = PagedCache(model, requests=6, tokens=600, page_size=16)
+    together = generate(model, prompts, 20, cache=cache)
+    end = together.tokens[1][4]
+    cut = generate(model, prompts, 20, cache=cache, end_token=end)
+    assert cache.held == [0] * 6 and int(cache.free_count) == cache.free.numel()
+    stops = [t.index(end) + 1 if end in t else 20 for t in together.tokens]
+    assert min(stops) < max(stops) - 3                          # of these inputs: some go on
+    for b, stop in enumerate(stops):
+        want, got = together.tokens[b][:stop], cut.tokens[b]
+        n = min(len(want), len(got))
+        differs = next((i for i in range(n) if want[i] != got[i]), None)
+        if differs is None:
+            assert len(want) == len(got)
+            assert max(abs(x - y) for x, y in zip(together.logprobs[b], cut.logprobs[b])) < (1e-4 if dev == "cpu" else 0.05)
+        else:
+            assert dev == "cuda" and abs(together.logprobs[b][differs] - cut.logprobs[b][differs]) < 0.05
