@@ -63,6 +63,24 @@ class PagedCache:
         self.lengths, self.free_count = ops.cache_release(mask, self.lengths, self.table, self.free, self.free_count, self.page_size)
         self.held = [0 if f else n for f, n in zip(finished, self.held)]
 
+    def take_back(self, tokens: Sequence[int]) -> None:
+        """Takes the last ``tokens[b]`` tokens of each request back (drafted ones that were rejected) and frees the pages behind what is left.  A page that
+        stays keeps the scale that they may have raised."""
+        if len(tokens) != self.requests or any(not 0 <= t <= n for t, n in zip(tokens, self.held)):
+            raise ValueError(f"a count of each request's tokens to take back is needed, of {self.held} at most")
+        left = [n - t for n, t in zip(self.held, tokens)]
+        keep, had = ([-(-n // self.page_size) for n in counts] for counts in (left, self.held))
+        there = lambda numbers, dtype: torch.tensor(numbers, dtype=dtype).to(self.lengths.device, non_blocking=True)  # noqa: E731
+        # the pages to free as requests of their own: each row of the table from the first of them on
+        W = self.table.shape[1]
+        at, first = torch.arange(W, device=self.table.device), there(keep, torch.long)[:, None]
+        tail = self.table.gather(1, (at + first).clamp(max=W - 1))
+        _, self.free_count = ops.cache_release(there([h > k for h, k in zip(had, keep)], torch.bool),
+                                               there([(h - k) * self.page_size for h, k in zip(had, keep)], torch.int32), tail, self.free, self.free_count,
+                                               self.page_size)
+        self.table.masked_fill_(at >= first, -1)
+        self.lengths, self.held = there(left, torch.int32), left
+
 
 class CacheStep:
     """One step's view of a :class:`PagedCache`: ``step[i]`` is what layer i appends to and attends over."""

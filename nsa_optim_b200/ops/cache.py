@@ -16,6 +16,9 @@ matrix instructions, so that a lane's 16 bytes are one load and nothing is trans
 Requests share the pages: ``table`` (B, W) int32 lists the pages of each request in order, ``free`` int32 and ``free_count`` (1) are a stack
 of the pages that nobody holds.  The new tokens of a step are packed one request after another, N in all; ``query_start`` (B + 1) int32 says
 where each begins, ``lengths`` (B) int32 how many tokens it has in the cache with them.
+
+A request holds the pages of its first ceil(lengths / P) entries of ``table``; entries behind them count as empty, whatever is in them.  So who lowers a length
+(drafted tokens that were rejected) gives the pages behind it back first, as ``generation.PagedCache.take_back`` does.
 """
 from __future__ import annotations
 

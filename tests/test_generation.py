@@ -332,3 +332,58 @@ def test_requests_go_on_when_others_end(dev):
             assert max(abs(x - y) for x, y in zip(together.logprobs[b], cut.logprobs[b])) < (1e-4 if dev == "cpu" else 0.05)
         else:
             assert dev == "cuda" and abs(together.logprobs[b][differs] - cut.logprobs[b][differs]) < 0.05
+
+
+def test_drafts_are_taken_back(dev):
+    """Tokens that are verified and rejected leave the cache with their pages; none is lost, and what follows agrees with the whole text (the bound of
+    test_steps_agree_with_the_whole_text: codes may have been rounded once more where a rejected token raised a page's scale)."""
+    model = small(dev)
+    ids = texts([100, 60, 80])
+    cache = PagedCache(model, requests=3, tokens=260, page_size=16)
+    at, gen = [0, 0, 0], torch.Generator().manual_seed(5)
+    for turn, (right, drafted) in enumerate((([30, 16, 1], [0, 0, 0]), ([1, 1, 15], [17, 15, 1]), ([1, 0, 16], [3, 0, 33]), ([0, 31, 1], [0, 16, 0]),
+                                             ([1, 1, 1], [40, 0, 0]), ([20, 1, 20], [5, 5, 5]))):
+        packed = []
+        for b in range(3):
+            packed += ids[b][at[b]:at[b] + right[b]] + torch.randint(0, 512, (drafted[b],), generator=gen).tolist()
+        new = [r + d for r, d in zip(right, drafted)]
+        with torch.no_grad():
+            logits = model(torch.tensor([packed], device=dev), past_key_values=cache.step(new))[0][0]
+        row = 0
+        for b in range(3):
+            if right[b]:
+                assert off(logits[row:row + right[b]], whole(model, ids[b], dev)[at[b]:at[b] + right[b]]) < 0.1
+            row += new[b]
+            at[b] += right[b]
+        cache.take_back(drafted)
+        assert cache.held == cache.lengths.tolist() == at
+        held = [-(-n // 16) for n in at]
+        table = cache.table.tolist()
+        assert all(p == -1 for b in range(3) for p in table[b][held[b]:])
+        pages = [p for b in range(3) for p in table[b][:held[b]]] + cache.free[:int(cache.free_count)].tolist()
+        assert sorted(pages) == list(range(cache.free.numel()))
+    cache.take_back(at)
+    assert cache.held == [0, 0, 0] and int(cache.free_count) == cache.free.numel()
+
+
+def test_refused_drafts(dev):
+    cache = PagedCache(small(dev, layers=1), requests=2, tokens=64)
+    cache.step([5, 0])
+    before = state_of(cache)
+    for counts in ([6, 0], [0, 1], [-1, 0], [1], [1, 0, 0]):
+        with pytest.raises(ValueError):
+            cache.take_back(counts)
+    assert state_of(cache) == before
+
+
+@pytest.mark.gpu
+def test_taking_drafts_back_does_not_wait(native):
+    cache = PagedCache(small("cuda", layers=1), requests=2, tokens=640)
+    cache.step([100, 70])
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        cache.take_back([50, 0])
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert cache.lengths.tolist() == [50, 70]
