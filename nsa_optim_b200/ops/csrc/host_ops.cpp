@@ -1304,12 +1304,13 @@ OP(cache_attention) {                            // q, pages, step, window, scal
            " heads, ", p.D, "), got ", q_.sizes());
       WANT(window >= 0, "window has to be 0 (none) or more");
       const Tensor q = packed_rows(q_), o = alloc(q.sizes(), BF, dev);
-      const long far = std::numeric_limits<int>::max();
+      // a window beyond every position is none: the kernel takes it off positions, which begin at -(tokens) and are met 64 keys at a time
+      const long far = std::numeric_limits<int>::max(), widest = far - q.size(0) - 64;
       const int new_ = dim(most < 1 ? 1 : most < far ? most : far), Hq = small(q.size(1), "the number of heads");
       const Tensor scratch = alloc({have(lib.nsa_cache_attention_scratch)(Hq, p.H, p.D, new_)}, F32, dev);
       launch(lib.nsa_cache_attention, static_cast<const void*>(ptr(q)), q.stride(0), static_cast<const void*>(ptr(p.k)),
              static_cast<const void*>(ptr(p.v)), fp(p.scale), ip(s.table), ip(s.start), ip(s.lengths), ptr(o), fp(scratch), s.B(),
-             s.W(), small(q.size(0), "the number of tokens"), p.n, Hq, p.H, p.D, p.P, window < far ? dim(window) : 0, scale, new_);
+             s.W(), small(q.size(0), "the number of tokens"), p.n, Hq, p.H, p.D, p.P, window <= widest ? dim(window) : 0, scale, new_);
       return o;
     };
   });

@@ -652,3 +652,13 @@ def test_a_token_that_takes_nearly_all(native, Hq):
     others = torch.arange(L - n, L, dtype=torch.double)
     want = (others / (others + math.exp(16.875)))[:, None, None]
     assert ((got - want).abs() <= want * (2.0 ** -8 + 2.0 ** -10)).all(), (got[0, 0, 0], want[0], got[-1, -1, -1], want[-1])
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 2, 2 ** 31 - 40, 2 ** 31 - 1, 2 ** 40])
+def test_windows_that_hold_everything(dev, window):
+    """The largest windows, also where a request is given more queries than it has tokens: the first of them see nothing."""
+    gen = torch.Generator().manual_seed(16)
+    lengths, new = [5, 70, 20], [9, 3, 30]
+    c, table = filled(dev, gen, lengths, 2, 64, 16)
+    got = attend(c, some(gen, 42, 8, 64, dev), table, new, lengths, window)
+    assert not got[:4].any() and got[4:12].flatten(1).any(1).all() and not got[12:22].any() and got[22:].flatten(1).any(1).all()
