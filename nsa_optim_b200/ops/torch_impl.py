@@ -435,7 +435,7 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top_k: int = 0, ignore_index:
     S = torch.where(empty, 1.0, e.sum(-1, keepdim=True))
     logp = below - S.log()
     p = e / S
-    gone = torch.isneginf(x)
+    gone = e == 0                                              # their log probability may be as large as the type holds
     entropy = -(p * torch.where(gone, 0.0, logp)).masked_fill(gone, 0.0).sum(-1)
     counts = (tokens != ignore_index) & (tokens >= 0) & (tokens < x.shape[-1])
     chosen = logp.gather(-1, torch.where(counts, tokens, 0).unsqueeze(-1)).squeeze(-1)

@@ -331,3 +331,13 @@ def test_refusals(dev, change):
     t = change["tokens"](x, tok) if "tokens" in change else tok
     with pytest.raises(ValueError):
         ops.token_logprobs(a, t, k)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_entropy_gradient_beside_masked_logits(dev, dtype):
+    """A token of probability 0 has no part in the gradient, however large the entropy's is: its log probability times that may be infinite."""
+    gen = torch.Generator().manual_seed(12)
+    x = logits(gen, 4, 300, dtype, "cpu")
+    x[:, 100:] = torch.finfo(dtype).min
+    g = grads_of(gen, 4, 3, dev)
+    check(x.to(dev), tokens_of(gen, 4, 300, dev), 3, grads=(g[0], torch.tensor([1.5, -40.0, 1e3, 2.0], device=dev), g[2]))
