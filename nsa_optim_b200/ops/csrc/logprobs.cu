@@ -44,7 +44,9 @@ constexpr int kBuffer = 480;              // candidates for them
 constexpr int kParts = 8;                 // CTAs of a cluster
 constexpr int kWidest = 32767 * kThreads * kUnroll * 4;      // columns: halves of chunks are counted in 16 bits
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLow = -1e30f;            // logits below it count as this in the pass: 2^-inf times -inf is no number
+// Logits below -kFar count as it in the pass, and rows whose maximum is above kFar or within a factor of ten of -kFar are looked at again at their end: R's rounding
+// is 4 at most then, so that S, which has 2 to the power of it, is a number.  (With -1e30 for it, stretches of masks of -1e10 and the like made rows NaN.)
+constexpr float kFar = 0x1p26f, kLow = -kFar;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -103,7 +105,7 @@ struct Vec<bf16> {
   static __device__ __forceinline__ uint4 pack(const float2 (&x)[4]) { return make_uint4(two(x[0]), two(x[1]), two(x[2]), two(x[3])); }
   __device__ __forceinline__ void clear() { w = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
   __device__ __forceinline__ void floats(float2 (&x)[4]) const {       // none below kLow
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w}, low = 0xf149f149u;     // bf16 of -1e30
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w}, low = 0xcc80cc80u;     // bf16 of kLow
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t c = max2_nan(v[i], low);
@@ -463,7 +465,7 @@ __device__ __noinline__ void finish(const u64* lists, Sums a, const T* x, long r
   const int lane = threadIdx.x & 31;
   float m = a.m, logS = logf(a.S) - fmaf(m, kLog2e, -a.R) * kLn2, H = logf(a.S);
   bool empty = false;
-  if (m <= 0.1f * kLow) {                                              // near kLow the pass has not told logits apart
+  if (m <= 0.1f * kLow || m > kFar) {                                  // the pass has not told logits apart, or its sums are none
     m = -CUDART_INF_F;
     for (int c = lane; c < V; c += 32) m = max_nan(m, value(x, c));
     for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));

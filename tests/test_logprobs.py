@@ -341,3 +341,24 @@ def test_entropy_gradient_beside_masked_logits(dev, dtype):
     x[:, 100:] = torch.finfo(dtype).min
     g = grads_of(gen, 4, 3, dev)
     check(x.to(dev), tokens_of(gen, 4, 300, dev), 3, grads=(g[0], torch.tensor([1.5, -40.0, 1e3, 2.0], device=dev), g[2]))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("size", [1e7, 1e8, 1e9, 1e10, 7e12, 1e20, 1e30, 3e38])
+@pytest.mark.parametrize("V", [5003, 40009])
+def test_logits_far_from_zero(dev, dtype, size, V):
+    """Masks of any size in whole stretches of the columns, single logits as large, rows that lie far from zero as a whole."""
+    gen = torch.Generator().manual_seed(11)
+    x = logits(gen, 8, V, dtype, "cpu")
+    x[0, :V // 2] = -size
+    x[1, V // 2:] = -size
+    x[2, 700:] = -size
+    x[2, :700] = -size / 2
+    x[3, 4000] = size
+    x[4, [3, V - 3]] = size
+    x[5] = size
+    x[6] = -size
+    x[7] = -size
+    x[7, V // 3] = 5.0
+    tok = torch.tensor([V - 2, 5, 3, 4000, V - 3, 17, 18, V // 3])
+    check(x.to(dev), tok.to(dev), 6, grads=grads_of(gen, 8, 6, dev))
