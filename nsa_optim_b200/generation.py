@@ -6,7 +6,8 @@
 
 A step takes any mix of prompts, single tokens and idle requests, packed one request after another: ``ops.cache_plan`` finds pages and
 slots, each layer appends its keys and values (``ops.cache_append``) and attends over the pages (``ops.cache_attention``), and
-``ops.token_logprobs`` turns the logits into the chosen tokens' log probabilities.  Nothing but the end of a request (an end token) makes the host wait.
+``ops.token_logprobs`` turns the logits into the chosen tokens' log probabilities.  Nothing but the end of a request (an end token) makes the host wait
+for a bf16 model on a GPU; models of other types append and attend in PyTorch there, which waits in every layer.
 The reference decodes with a concatenated cache (models/transformer.py:104-118 there); that path is still ``use_cache=True``.
 
     python -m nsa_optim_b200.generation --requests 16 --prompt_length 512 --max_new_tokens 64

@@ -299,8 +299,9 @@ def cache_release(finished: Tensor, lengths: Tensor, table: Tensor, free: Tensor
 
 def cache_append(pages: KVPages, k: Tensor, v: Tensor, table: Tensor, query_start: Tensor, lengths: Tensor) -> None:
     """Rounds the keys and values (N, Hkv, D) of a step's packed tokens to 8 bits and stores them, in place, as the last
-    ``query_start[b + 1] - query_start[b]`` of each request's ``lengths[b]`` tokens.  A page's first token sets its scale anew; larger values raise it later,
-    and the page's codes with it.  Tokens without a page are left out, and so are rows of no request (before ``query_start[0]`` or from ``query_start[B]`` on)."""
+    ``query_start[b + 1] - query_start[b]`` of each request's ``lengths[b]`` tokens.  bf16 on a GPU is a kernel; other types run in PyTorch, request by
+    request, and wait for the device.  A page's first token sets its scale anew; larger values raise it later, and the page's codes with it.  Tokens without a
+    page are left out, and so are rows of no request (before ``query_start[0]`` or from ``query_start[B]`` on)."""
     if _use_native(k, "cache"):
         return native_module().cache_append(pages, k, v, table, query_start, lengths)
     return cache.append(pages, k, v, table, query_start, lengths)
@@ -319,7 +320,8 @@ def cache_attention(q: Tensor, pages: KVPages, table: Tensor, query_start: Tenso
     """Causal attention of packed queries (N, Hq, D), the last ``query_start[b + 1] - query_start[b]`` of each request's ``lengths[b]`` tokens, over the
     request's cached keys and values, their own among them (``window`` > 0: the last ``window`` of these alone).  Query heads share KV heads in equal
     groups.  A query that sees nothing gets zeros, and so does a row of no request, before ``query_start[0]`` or from ``query_start[B]``
-    on.  ``max_new``, the most queries of a request, is a hint for the split of the work: any value gives the same sums up to their order.  Inference only: no gradient is recorded."""
+    on.  ``max_new``, the most queries of a request, is a hint for the split of the work: any value gives the same sums up to their order.  Inference only: no
+    gradient is recorded.  bf16 with a head_dim of 64 or 128 on a GPU is a kernel; the rest runs in PyTorch, request by request, and waits for the device."""
     if _use_native(q, "cache"):
         return native_module().cache_attention(q, pages, table, query_start, lengths, window, scale, max_new)
     return cache.attention(q.detach(), pages, table, query_start, lengths, window, scale)
@@ -329,7 +331,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top_k: int = 0, ignore_index:
     """Of logits (..., V): the log probability of each given token (0 where it is ``ignore_index`` or no token), the entropy of each
     distribution, and the ``top_k`` likeliest tokens with their log probabilities (equal logits: the lower index first), all fp32 and
     differentiable with respect to the logits.  Tokens whose logit is -inf have probability 0; where no token is left, log
-    probabilities are -inf, the entropy is 0 and no gradient flows."""
+    probabilities are -inf, the entropy is 0 and no gradient flows.  bf16 and fp32 on a GPU are kernels up to ``top_k`` of 32; beyond, PyTorch sorts the
+    rows (counted by ``native.fallback_counts``)."""
     if logits.is_cuda and _BACKEND != "torch" and logits.dtype in (torch.bfloat16, torch.float32):
         return native_module().token_logprobs(logits, tokens, top_k, ignore_index)
     return torch_impl.token_logprobs(logits, tokens, top_k, ignore_index)

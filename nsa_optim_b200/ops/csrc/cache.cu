@@ -9,7 +9,7 @@ typedef __nv_bfloat16 bf16;
 
 // ------------------------------------------------------------------------------------- pages and slots of a step
 // A few thousand numbers at most: what counts is the chain of dependent loads (lengths and counts together, then a page number) and barriers, so each
-// CTA scans all requests by itself and no CTA waits for another.  64 requests of one token 3.5 us, 512 requests with 65 K tokens 5.1 us.
+// CTA scans all requests by itself and no CTA waits for another.  64 requests of one token 3.3 us, 512 requests with 65 K tokens 4.8 us.
 constexpr int kPlanThreads = 1024;
 
 // Exclusive prefix of a value per thread over the CTA, and the total
@@ -492,6 +492,8 @@ extern "C" int nsa_cache_plan(const int* lengths, const int* add, int* table, co
     const cudaError_t e = cudaFuncSetAttribute(cache_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200000);
     if (e != cudaSuccess) return nsa::fail_cuda(e, "nsa_cache_plan");
   }
+  // as many threads as requests, up to 1024: fewer scan in turns, more wait for one another.  One token each, with 128 / 512 / 1024 threads: 64 requests 3.3 / 3.5 /
+  // 4.1 us, 256 4.5 / 3.8 / 4.4, 512 6.6 / 4.1 / 4.7, 4096 34.7 / 12.9 / 11.1 (65536 tokens of 64 requests, which write more than they scan: 5.8 / 4.4 / 5.5)
   const int threads = B <= 128 ? 128 : B <= 512 ? 512 : kPlanThreads;
   const int want = (N + threads - 1) / threads, most = nsa::sm_count();
   const int grid = want < 1 ? 1 : want < most ? want : most;
@@ -520,7 +522,11 @@ extern "C" int nsa_cache_append(const void* k, const void* v, long ldk, long ldv
   if (B <= 0 || H <= 0 || H > 65535 || D % 64 || N < 0) return nsa::fail(NSA_ERR_SHAPE, "cache_append: unsupported shape");
   const CachePages c{static_cast<uint8_t*>(kc), static_cast<uint8_t*>(vc), scale, pages, H, D, __builtin_ctz(page_size)};
   const CacheStep s{table, query_start, lengths, B, W, N};
-  // few tokens: one a CTA, most of them the first of their page; else a page's worth.  Warps for the 16-token blocks of a page
+  // Up to 2048 tokens: one a CTA, which passes over all but a group's first; else a page's worth, since for long groups those CTAs cost more than they do, while
+  // a window of single tokens takes them one after another.  Pages of 64, 8 heads of 128, a token / a page's worth a CTA: 64 requests of one token 7.5 / 263 us, 512
+  // 18.6 / 289, 2048 62.8 / 351, 64 requests of 8 13.6 / 35; 4 of 512 23.3 / 9.4, 4 of 1024 40 / 10.5, 8 of 4096 277 / 41.  More than 2048 single tokens are on the
+  // wrong side of it (4096 122 / 360).  Warps for the 16-token blocks of a page; one where a group can have only one (512 requests 18.6
+  // us, with as many as the page has blocks 34)
   const int window = N <= 2048 ? 1 : page_size, C = D % 128 ? 2 : 4, blocks = page_size / 16 * (D / (32 * C));
   const int warps = window == 1 && N <= B ? 1 : blocks < 16 ? blocks : 16;
   const dim3 grid((N + window - 1) / window, H, 2);

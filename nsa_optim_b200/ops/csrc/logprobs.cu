@@ -15,7 +15,8 @@
 // where each CTA has one row, nothing hides its end, and its instructions come from memory the first time (8 in about 50 cycles of a lone warp); where
 // it has many, they share the issue slots.  So loops stay loops, maxima are ranked by counting, and a single token's bound is one maximum.
 //
-// Measured: 4096 x 151936 bf16, k = 8: 235 us, 5.3 TB/s (backward 371 us, 6.7 TB/s, some of it from L2); 8192 x 32000, k = 1: 116 us, 4.5 TB/s; 511 x 50257 fp32, k = 5: 28 us;
+// Measured, kernels alone: 4096 x 151936 bf16, k = 8: 232 us, 5.4 TB/s (backward 371 us, 6.7 TB/s, some of it from L2); 8192 x 32000, k = 1: 114 to 116 us, 4.5 TB/s; 511 x 50257
+// fp32, k = 5: 26 to 28 us;
 // 64 x 151936, k = 20: 19 us, of which 5.5 to 7 until the last logit has been seen, 4.5 for the candidates, 2 for the slowest CTA of a cluster, 2 for places.
 //
 // Compiled without fast math: the logarithms at a row's end are the exact ones, the exponentials of its elements the hardware's.
@@ -630,7 +631,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtas) logprobs_fwd_kernel(cons
 }
 
 // dx_j = -p_j (G + g_H (log p_j + H)), G the sum of the row's other gradients; theirs are added at their tokens.  One CTA per kBwdPieces pieces of a row.
-// Bytes bound it, and how they are asked for: 4096 x 151936 bf16, forward and backward, with 8 loads of each of 128 threads 606 us, 8 of 96, 160, 192 and 256
+// Bytes bound it, and how they are asked for: 4096 x 151936 bf16, forward and backward in turn on the same memory, with 8 loads of each of 128 threads 606 us, 8 of 96, 160, 192 and 256
 // 608, 610, 632 and 652, 4 of 256 667, 7 and 9 of 128 622, 16 of 64 772; loads that leave the caches first 618, stores that do not 617; rows from the
 // first on, not from the last, which the forward pass has left in L2, 608.
 constexpr int kBwdThreads = 128, kBwdTurns = 8, kBwdPieces = kBwdThreads * kBwdTurns;
@@ -709,7 +710,10 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(const T* __re
 template <class T>
 cudaError_t forward(const void* logits, long ld, const long long* tokens, float* logprob, float* entropy, float* stats, float* top, long long* index,
                     long rows, int V, int k, long long ignore, cudaStream_t st) {
-  // CTAs of a row: with fewer rows than SMs up to 8, of 4096 columns at least
+  // CTAs of a row: up to 8 where the GPU holds them all at once, of 4096 columns at least: a cluster's start and end cost about 1.5 us, a CTA reads 9000 columns
+  // a us.  Rows of 8192 columns are faster whole, rows of 32000 in more parts; one row, k = 1, in parts of 4096 / 8192 / 16384 columns at least / whole: 8192
+  // columns 8.0 / 6.7 / 6.6 / 6.7 us, 16384 8.6 / 8.3 / 7.7 / 7.9, 32000 8.7 / 9.3 / 9.9 / 9.9, 50257 9.9 / 10.6 / 11.9 / 13.0, 151936 10.7 / 10.7 / 10.7 / 22.7; 64 rows, k = 20:
+  // 8192 10.3 / 8.4 / 8.7 / 8.4, 32000 11.7 / 11.9 / 13.2 / 13.8, 151936 18.2 / 18.5 / 18.3 / 34.7
   const int sms = nsa::sm_count();
   int parts = 1;
   while (parts < kParts && rows * parts * 2 <= static_cast<long>(kCtas) * sms && V / (2 * parts) >= 4096) parts *= 2;
