@@ -88,6 +88,7 @@ class CacheStep:
 
     def __init__(self, cache: PagedCache, plan: ops.CachePlan, max_new: int):
         self.cache, self.plan, self.max_new = cache, plan, max_new
+        self.limit = max(cache.held)                         # above all of the plan's positions, whatever leaves the cache later
         self._rotary: dict = {}
 
     def __getitem__(self, layer: int) -> "LayerStep":
@@ -101,7 +102,7 @@ class CacheStep:
         """Cosines and sines of the step's positions, looked up once for all layers."""
         key = (emb.dim, emb.base)
         if key not in self._rotary:
-            self._rotary[key] = emb.rows(self.plan.positions, max(self.cache.held))
+            self._rotary[key] = emb.rows(self.plan.positions, self.limit)
         return self._rotary[key]
 
 

@@ -387,3 +387,14 @@ def test_taking_drafts_back_does_not_wait(native):
     finally:
         torch.cuda.set_sync_debug_mode("default")
     assert cache.lengths.tolist() == [50, 70]
+
+
+def test_a_step_knows_its_positions(dev):
+    """A step whose requests have left the cache when it runs: its tokens are stored nowhere, and no row behind the rotary tables is asked for."""
+    model = small(dev, layers=1)
+    cache = PagedCache(model, requests=2, tokens=400)
+    step = cache.step([300, 0])                                # the model's tables have 256 rows
+    cache.release([True, False])
+    with torch.no_grad():
+        h = model(torch.tensor(texts([300]), device=dev), past_key_values=step, return_hidden=True)[0]
+    assert h.isfinite().all()
