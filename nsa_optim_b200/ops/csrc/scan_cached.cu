@@ -168,7 +168,16 @@ __device__ __forceinline__ float ex2(float x) {                        // two st
 
 // Numbers of a chunk and head, by a warp, four neighbouring tokens a lane: what both kernels need of the step sizes is worked out once.  (With these sums in a
 // warp of the kernels themselves its 600 instructions took longer than everything beside them: 3000 cycles a chunk in both.)  It does not wait for the plan.
-constexpr int kCum = 0, kLess = L, kCols = 2 * L, kRowFloats = 2 * L + 192, kWeight = kRowFloats, kDecay = kWeight + L, kRecord = kDecay + 4;
+// The sums of a chunk's logarithms are kept in two fp32 numbers each, formed in 64 bits: rows need differences of them, of which long steps in front would take the
+// bits (in one number a token's own weight, its step size, was off by 0.5 % at steps of 60 and decays of 16).  Decays of less than 2^-kMostDecay are that: all that
+// they multiply, a weight of 2^128 at most, is zero in fp32 either way, and the sums stay finite for any step size.
+constexpr float kMostDecay = 512.f;
+constexpr int kCum = 0, kLess = L, kCumLow = 2 * L, kLessLow = 3 * L, kCols = 4 * L, kRowFloats = 4 * L + 192, kWeight = kRowFloats, kDecay = kWeight + L,
+              kRecord = kDecay + 4;
+__device__ __forceinline__ float rest_of(double x) {                   // what the number rounded to fp32 leaves
+  const float high = static_cast<float>(x);
+  return isfinite(high) ? static_cast<float>(x - high) : 0.f;
+}
 __device__ __forceinline__ void chunk_numbers(const Scan& a, const Plan& plan, int longest, int c, int h) {
   const int lane = threadIdx.x & 31, blk = lane >> 3;
   const float rate = -expf(param(a.A_log, h, a.A_fp32)) * LOG2E, bias = param(a.bias, h, a.bias_fp32);
@@ -182,33 +191,41 @@ __device__ __forceinline__ void chunk_numbers(const Scan& a, const Plan& plan, i
     for (int i = 0; i < 4; ++i) {                      // 0 behind the request's last token
       d[i] = 4 * lane + i < chunk.y ? softplus(raw[i] + bias) : 0.f;
       v[i] = d[i] * rate;
+      if (v[i] < -kMostDecay) v[i] = -kMostDecay;      // NaN stays
     }
     // inclusive sums from the chunk's start, exclusive ones from its end, in units of log 2
-    float up[4] = {v[0], v[0] + v[1], v[0] + v[1] + v[2], v[0] + v[1] + v[2] + v[3]}, down[4] = {v[3] + v[2] + v[1], v[3] + v[2], v[3], 0.f};
-    float run = up[3], back = up[3];
+    double up[4] = {v[0], static_cast<double>(v[0]) + v[1], 0., 0.};
+    up[2] = up[1] + v[2], up[3] = up[2] + v[3];
+    float down[4] = {v[3] + v[2] + v[1], v[3] + v[2], v[3], 0.f};
+    double run = up[3];
+    float back = down[0] + v[0];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const float x = __shfl_up_sync(0xffffffffu, run, o), y = __shfl_down_sync(0xffffffffu, back, o);
+      const double x = __shfl_up_sync(0xffffffffu, run, o);
+      const float y = __shfl_down_sync(0xffffffffu, back, o);
       if (lane >= o) run += x;
       if (lane + o < 32) back += y;
     }
-    float before = __shfl_up_sync(0xffffffffu, run, 1), behind = __shfl_down_sync(0xffffffffu, back, 1);
-    if (lane == 0) before = 0.f;
+    double before = __shfl_up_sync(0xffffffffu, run, 1);
+    float behind = __shfl_down_sync(0xffffffffu, back, 1);
+    if (lane == 0) before = 0.;
     if (lane == 31) behind = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) up[i] += before, down[i] += behind;
     float* to = plan.records() + (static_cast<long>(c) * a.H + h) * kRecord;
-    *reinterpret_cast<float4*>(to + kCum + 4 * lane) = make_float4(up[0], up[1], up[2], up[3]);
-    *reinterpret_cast<float4*>(to + kLess + 4 * lane) = make_float4(up[0] - log2f(d[0]), up[1] - log2f(d[1]), up[2] - log2f(d[2]), up[3] - log2f(d[3]));
+    auto keep = [&](int high, int low, const double (&x)[4]) {
+      *reinterpret_cast<float4*>(to + high + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(to + low + 4 * lane) = make_float4(rest_of(x[0]), rest_of(x[1]), rest_of(x[2]), rest_of(x[3]));
+    };
+    keep(kCum, kCumLow, up);
+    keep(kLess, kLessLow, {up[0] - log2f(d[0]), up[1] - log2f(d[1]), up[2] - log2f(d[2]), up[3] - log2f(d[3])});
     // Pairs of rows in different blocks of 32 need no exponential of their own: with m the sum at the end of an earlier block, exp(c_i - c_j) = exp(c_i - m)
     // exp(m - c_j), and both exponents are <= 0: the factors of columns j for row block p + 1, j < 32 (p + 1), at 16 p (p + 1) + j
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
-      const float mid = __shfl_sync(0xffffffffu, up[3], 8 * p + 7);
-      if (blk <= p)
-        *reinterpret_cast<float4*>(to + kCols + 16 * p * (p + 1) + 4 * lane) =
-            make_float4(ex2(fminf(mid - up[0], 0.f)) * d[0], ex2(fminf(mid - up[1], 0.f)) * d[1], ex2(fminf(mid - up[2], 0.f)) * d[2],
-                        ex2(fminf(mid - up[3], 0.f)) * d[3]);
+      const double mid = __shfl_sync(0xffffffffu, up[3], 8 * p + 7);
+      auto factor = [&](int i) { return ex2(fminf(static_cast<float>(mid - up[i]), 0.f)) * d[i]; };
+      if (blk <= p) *reinterpret_cast<float4*>(to + kCols + 16 * p * (p + 1) + 4 * lane) = make_float4(factor(0), factor(1), factor(2), factor(3));
     }
     *reinterpret_cast<float4*>(to + kWeight + 4 * lane) =
         make_float4(d[0] * exp2f(down[0]), d[1] * exp2f(down[1]), d[2] * exp2f(down[2]), d[3] * exp2f(down[3]));
@@ -705,11 +722,11 @@ scan_rows_kernel(const __grid_constant__ CUtensorMap tm_c, const __grid_constant
       }
       if (!before && buf != own) continue;
       if (!wait(full + k % kStages, k / kStages, STATUS_TIMEOUT_SMEM_FULL)) break;
-      const float *cum = sums + k % kStages * kRowFloats + kCum, *cumd = cum + kLess - kCum, *colf = cum + kCols - kCum;
-      const float ci = cum[r];
+      const float *cum = sums + k % kStages * kRowFloats + kCum, *low = cum + kCumLow - kCum, *colf = cum + kCols - kCum;
+      const float ci = cum[r], ci_low = low[r];
       uint32_t pk[16];
       if (before) {                                    // every column is before every row
-        const float rowf = ex2(fminf(ci - cum[32 * quad - 1], 0.f));
+        const float rowf = ex2(fminf((ci - cum[32 * quad - 1]) + (ci_low - low[32 * quad - 1]), 0.f));
         const float2 r2 = make_float2(rowf, rowf);
         const float* f = colf + 16 * quad * (quad - 1) + grp * 32;
 #pragma unroll
@@ -721,10 +738,11 @@ scan_rows_kernel(const __grid_constant__ CUtensorMap tm_c, const __grid_constant
           pk[j / 2 + 1] = tc5::pack_bf16(y.x, y.y);
         }
       } else {
-        const float2 c2 = make_float2(ci, ci), minus = make_float2(-1.f, -1.f);
+        const float2 c2 = make_float2(ci, ci), low2 = make_float2(ci_low, ci_low), minus = make_float2(-1.f, -1.f);
+        const float *less = cum + kLess - kCum + grp * 32, *less_low = cum + kLessLow - kCum + grp * 32;
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {              // exponents are <= 0 where they count
-          const float2 x = fma2(*reinterpret_cast<const float2*>(cumd + grp * 32 + j), minus, c2);
+        for (int j = 0; j < 32; j += 2) {              // exponents are <= 0 but for the step size where they count
+          const float2 x = add2(fma2(*reinterpret_cast<const float2*>(less + j), minus, c2), fma2(*reinterpret_cast<const float2*>(less_low + j), minus, low2));
           const float2 v = mul2(make_float2(s[j], s[j + 1]), make_float2(ex2(x.x), ex2(x.y)));
           pk[j / 2] = tc5::pack_bf16(j <= lane ? v.x : 0.f, j + 1 <= lane ? v.y : 0.f);
         }

@@ -94,7 +94,7 @@ def scan(x: Tensor, dt: Tensor, A_log: Tensor, Bm: Tensor, Cm: Tensor, D: Option
     y = torch.zeros_like(x, memory_format=torch.contiguous_format)
     start, total, rep = query_start.tolist(), lengths.tolist(), x.shape[1] // Bm.shape[1]
     step = F.softplus(dt.detach().float() + dt_bias.detach().float())
-    log_decay = step * -torch.exp(A_log.detach().float())
+    log_decay = (step * -torch.exp(A_log.detach().float())).clamp(min=-1000.0)       # a decay of zero either way, and sums of them that stay finite
     for b, (lo, hi) in enumerate(zip(start, start[1:])):
         lo, hi, new = max(lo, 0), min(hi, x.shape[0]), hi - lo
         if hi <= lo:
