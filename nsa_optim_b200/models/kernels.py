@@ -151,11 +151,14 @@ def rotate_half(x: Tensor) -> Tensor:
 
 
 def apply_rotary_pos_emb(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, interleaved: bool = False) -> Tuple[Tensor, Tensor]:
-    """q, k (B, T, H, D); cos/sin (T, R/2) for the first R columns of a head (or (T, D) with duplicated halves)."""
+    """q, k (B, T, H, D); cos/sin (T, R/2) for the first R columns of a head (or (T, D) with duplicated halves), a row a token."""
     d2 = q.shape[-1] // 2
     if cos.shape[-1] == q.shape[-1]:
         cos, sin = cos[..., :d2], sin[..., :d2]
-    if q.dtype == torch.bfloat16 or interleaved or cos.shape[-1] != d2:
+    apart = interleaved or cos.shape[-1] != d2
+    if apart and cos.shape[0] != q.shape[1]:
+        raise ValueError(f"cos and sin have to have a row for each of {q.shape[1]} tokens, got {tuple(cos.shape)}")
+    if apart or (q.dtype == k.dtype == torch.bfloat16 and q.shape[:2] == k.shape[:2] and cos.shape[0] == q.shape[1]):
         return ops.rope_qk(q, k, cos, sin, None, interleaved)
     return ops.rope(q, cos, sin), ops.rope(k, cos, sin)
 

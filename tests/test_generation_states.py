@@ -299,3 +299,16 @@ def test_options_of_the_command_line():
         model = build_model(build_training_config(args), args, verbose=False)[0]
         emb = [m for m in model.modules() if isinstance(m, RotaryEmbedding)]
         assert emb and all((m.dim, m.scaling, m.interleaved) == (32, "yarn:4:16", True) for m in emb)
+
+
+def test_rotary_calls_of_one_side_at_a_time(dev):
+    """Queries and keys that one launch cannot take together are turned as each of them alone, and rows that do not fit the tokens are refused, not passed over."""
+    emb = RotaryEmbedding(64, 64, 1e4)
+    q, k = torch.randn(2, 9, 3, 64, device=dev).to(torch.bfloat16), torch.randn(2, 9, 1, 64, device=dev).to(torch.bfloat16)
+    cos, sin = emb(q)
+    for a, b, c, s in ((q, k, cos, sin), (q, k[:1], cos, sin), (q, k.float(), cos, sin), (q, k, cos[3:4], sin[3:4]), (q[:, :1], k, cos[:1], sin[:1])):
+        for got, x in zip(apply_rotary_pos_emb(a, b, c, s), (a, b)):
+            assert got.dtype == x.dtype and torch.equal(got, ops.rope(x, c, s))
+    for c, s, interleaved in ((cos[:5], sin[:5], False), (emb.cos_cached, emb.sin_cached, False), (cos[:5], sin[:5], True), (cos[:5, :8], sin[:5, :8], False)):
+        with pytest.raises((ValueError, RuntimeError)):
+            apply_rotary_pos_emb(q, k, c, s, interleaved)
