@@ -97,7 +97,7 @@ def residual_block(hidden: Tensor, norm1: nn.Module, mixer, norm2: nn.Module, ml
 
 class RotaryEmbedding(nn.Module):
     """cos/sin cache of shape (T, D/2) in fp32; grows on demand.  ``forward`` returns the
-    rows for ``position_ids`` (or the first ``seq_len`` rows).  ``dim`` is the number of a head's columns that are turned, ``scaling`` stretches the positions for
+    rows for ``position_ids``, (T) or (B, T), or the first ``seq_len`` rows; of ids (B, T), B other than 1, they are (B, T, D/2).  ``dim`` is the number of a head's columns that are turned, ``scaling`` stretches the positions for
     long contexts (``ops.rope_tables``), ``interleaved`` pairs neighbouring columns instead of the two halves."""
 
     def __init__(self, dim: int, max_position_embeddings: int = 2048, base: float = 10000.0, scaling: Optional[str] = None, interleaved: bool = False):
@@ -141,7 +141,11 @@ class RotaryEmbedding(nn.Module):
                                     device=x.device)
         if position_ids is None:
             return self.cos_cached[:need], self.sin_cached[:need]
-        pid = position_ids.reshape(-1)[: x.shape[1]] if position_ids.dim() > 1 else position_ids
+        pid = position_ids
+        if pid.dim() > 1:
+            if pid.dim() != 2 or pid.shape[0] not in (1, x.shape[0]):
+                raise ValueError(f"position_ids have to be (T), (1, T) or ({x.shape[0]}, T), got {tuple(pid.shape)}")
+            pid = (pid[0] if pid.shape[0] == 1 else pid)[..., : x.shape[1]]
         return self.cos_cached[pid], self.sin_cached[pid]
 
 
@@ -151,10 +155,14 @@ def rotate_half(x: Tensor) -> Tensor:
 
 
 def apply_rotary_pos_emb(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, interleaved: bool = False) -> Tuple[Tensor, Tensor]:
-    """q, k (B, T, H, D); cos/sin (T, R/2) for the first R columns of a head (or (T, D) with duplicated halves), a row a token."""
+    """q, k (B, T, H, D); cos/sin (T, R/2) for the first R columns of a head (or (T, D) with duplicated halves), a row a token; or (B, T, R/2), a row for each
+    sequence's token."""
     d2 = q.shape[-1] // 2
     if cos.shape[-1] == q.shape[-1]:
         cos, sin = cos[..., :d2], sin[..., :d2]
+    if cos.dim() == 3:
+        rows = torch.arange(cos.shape[0] * cos.shape[1], device=cos.device).view(cos.shape[:2])
+        return ops.rope_qk(q, k, cos.flatten(0, 1), sin.flatten(0, 1), rows, interleaved)
     apart = interleaved or cos.shape[-1] != d2
     if apart and cos.shape[0] != q.shape[1]:
         raise ValueError(f"cos and sin have to have a row for each of {q.shape[1]} tokens, got {tuple(cos.shape)}")

@@ -312,3 +312,41 @@ def test_rotary_calls_of_one_side_at_a_time(dev):
     for c, s, interleaved in ((cos[:5], sin[:5], False), (emb.cos_cached, emb.sin_cached, False), (cos[:5], sin[:5], True), (cos[:5, :8], sin[:5, :8], False)):
         with pytest.raises((ValueError, RuntimeError)):
             apply_rotary_pos_emb(q, k, c, s, interleaved)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_positions_of_each_sequence(dev, interleaved):
+    """Ids (B, T) turn each sequence by its own, as one call for each of them does; ids (1, T) and (T) turn all alike."""
+    dtype = torch.bfloat16 if dev == "cuda" else torch.float32
+    emb = RotaryEmbedding(32, 64, 1e4, interleaved=interleaved)
+    q, k = torch.randn(3, 9, 4, 64, device=dev).to(dtype), torch.randn(3, 9, 2, 64, device=dev).to(dtype)
+    ids = torch.stack([torch.arange(9), torch.arange(40, 49), torch.randint(0, 70, (9,))]).to(dev)
+    got = apply_rotary_pos_emb(q, k, *emb(q, ids), interleaved)
+    for b in range(3):
+        alone = apply_rotary_pos_emb(q[b:b + 1], k[b:b + 1], *emb(q[b:b + 1], ids[b]), interleaved)
+        assert all(torch.equal(x[b:b + 1], y) for x, y in zip(got, alone))
+    for same in (ids[1:2], ids[1], ids[1:2].expand(3, -1)):
+        for x, y in zip(apply_rotary_pos_emb(q, k, *emb(q, same), interleaved), apply_rotary_pos_emb(q, k, *emb(q, ids[1]), interleaved)):
+            assert torch.equal(x, y)
+    for bad in (ids[:2], ids[None]):
+        with pytest.raises(ValueError):
+            emb(q, bad)
+
+
+@pytest.mark.parametrize("hybrid", [False, True])
+def test_models_turn_each_sequence_by_its_own_positions(dev, hybrid):
+    """A batch whose second sequence begins at another position is two batches of one."""
+    if hybrid:
+        model = small(dev, "A")
+    else:
+        model = placed(create_model(ModelConfig(name="small", hidden_size=128, intermediate_size=256, num_hidden_layers=1, num_attention_heads=4,
+                                                num_key_value_heads=2, head_dim=64, vocab_size=256, max_position_embeddings=64)), dev)
+    tokens = torch.tensor([t[:24] for t in texts([24, 24], 256)], device=dev)
+    ids = torch.stack([torch.arange(24), 3 * torch.arange(24) + 5]).to(dev)       # steps of three: attention sees other distances
+    with torch.no_grad():
+        both = model(tokens, position_ids=ids)[0]
+        each = torch.cat([model(tokens[b:b + 1], position_ids=ids[b])[0] for b in range(2)])
+        other = model(tokens, position_ids=ids[0])[0]
+    assert off(both[1], other[1].float()) > 0.01
+    # the same sums in products of other shapes: fp32 of some hundred operations, or a few roundings of 2^-8 of activations and logits
+    assert off(both, each.float()) < (0.02 if dev == "cuda" else 1e-5)
