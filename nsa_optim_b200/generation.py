@@ -107,6 +107,7 @@ class CacheStep:
     def __init__(self, cache: PagedCache, plan: ops.CachePlan, max_new: int):
         self.cache, self.plan, self.max_new = cache, plan, max_new
         self.limit = max(cache.held)                         # above all of the plan's positions, whatever leaves the cache later
+        self._rotary: dict = {}
 
     def __getitem__(self, layer: int):
         state = self.cache.layers[layer]
@@ -116,17 +117,29 @@ class CacheStep:
         """Row of each request's last token in the packed step (that of the token before it where it has none)."""
         return (self.plan.query_start[1:] - 1).clamp(min=0).long()
 
+    def rotary(self, emb) -> Tuple[Tensor, Tensor]:
+        """Cosines and sines of the step's positions, looked up once for all layers: for queries and keys that are turned outside of ``attend``."""
+        key = (emb.dim, emb.base, getattr(emb, "scaling", None))
+        if key not in self._rotary:
+            self._rotary[key] = emb.rows(self.plan.positions, self.limit)
+        return self._rotary[key]
+
 
 class LayerStep:
     def __init__(self, step: CacheStep, pages: ops.KVPages):
         self.step, self.pages = step, pages
+        self.rotary = step.rotary
 
-    def attend(self, q: Tensor, k: Tensor, v: Tensor, rotary) -> Tensor:
+    def attend(self, q: Tensor, k: Tensor, v: Tensor, rotary=None) -> Tensor:
         """Attention of the step's packed queries (1, N, Hq, D) over their requests, to which k and v (1, N, Hkv, D) are appended first; queries and keys are turned
-        by their positions' rows of ``rotary``'s tables."""
+        by their positions' rows of ``rotary``'s tables, or come as they are (None)."""
         c, p = self.step.cache, self.step.plan
-        cos, sin = rotary.tables(self.step.limit, q.device)
-        q = ops.cache_append_rope(self.pages, q[0], k[0], v[0], cos, sin, c.table, p.query_start, p.lengths, rotary.interleaved)
+        q, k, v = q[0], k[0], v[0]
+        if rotary is None:
+            ops.cache_append(self.pages, k, v, c.table, p.query_start, p.lengths)
+        else:
+            cos, sin = rotary.tables(self.step.limit, q.device)
+            q = ops.cache_append_rope(self.pages, q, k, v, cos, sin, c.table, p.query_start, p.lengths, rotary.interleaved)
         return ops.cache_attention(q, self.pages, c.table, p.query_start, p.lengths, max_new=self.step.max_new).unsqueeze(0)
 
 

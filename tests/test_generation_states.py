@@ -350,3 +350,28 @@ def test_models_turn_each_sequence_by_its_own_positions(dev, hybrid):
     assert off(both[1], other[1].float()) > 0.01
     # the same sums in products of other shapes: fp32 of some hundred operations, or a few roundings of 2^-8 of activations and logits
     assert off(both, each.float()) < (0.02 if dev == "cuda" else 1e-5)
+
+
+@pytest.mark.parametrize("options", [{}, dict(scaling="linear:2"), dict(interleaved=True)])
+def test_layers_that_turn_by_themselves(dev, options):
+    """Rows of the step's positions, looked up by the step, and attention over what comes turned: the same as turning on the way in."""
+    model = small(dev, "A")
+    dtype = next(model.parameters()).dtype
+    emb = RotaryEmbedding(64, 64, 1e4, **options)
+    outs = []
+    for inside in (True, False):
+        torch.manual_seed(3)
+        cache = PagedCache(model, requests=2, tokens=100, page_size=16)
+        for new in ([20, 7], [1, 1]):
+            step = cache.step(new)
+            q, k, v = (torch.randn(1, sum(new), h, 64, device=dev).to(dtype) for h in (4, 2, 2))
+            if inside:
+                outs.append(step[0].attend(q, k, v, emb))
+            else:
+                cos, sin = step[0].rotary(emb)
+                assert torch.equal(cos, step.rotary(RotaryEmbedding(64, 64, 1e4, **options))[0]) and cos.shape == (sum(new), 32)
+                outs.append(step[0].attend(*apply_rotary_pos_emb(q, k, cos, sin, emb.interleaved), v))
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+    cache = PagedCache(model, requests=2, tokens=100, page_size=16)
+    step = cache.step([2, 2])
+    assert not torch.equal(step.rotary(RotaryEmbedding(64, 64, 1e4))[1], step.rotary(RotaryEmbedding(64, 64, 1e4, "linear:2"))[1])
