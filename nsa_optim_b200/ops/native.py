@@ -562,6 +562,7 @@ class _RoPEQK(torch.autograd.Function):
 def rope_qk(q, k, cos, sin, positions=None, interleaved=False):
     if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
         _fallback("rope", "the tables want a gradient")
+        torch_impl.check_rope_qk(q, k, cos, sin, positions)
         return torch_impl.rope_qk(q, k, cos, sin, positions, interleaved)
     return _run(_RoPEQK, q, k, cos, sin, positions, interleaved)
 

@@ -173,6 +173,18 @@ def test_refusals(dev):
             bad()
 
 
+def test_refusals_with_gradients_of_the_tables(dev):
+    """The same calls are refused where the tables want a gradient."""
+    cos, sin = (t.requires_grad_() for t in tables(64, 20, dev))
+    q, k = torch.randn(2, 5, 4, 64, device=dev).to(BF), torch.randn(2, 5, 2, 64, device=dev).to(BF)
+    for bad in (dict(positions=torch.zeros(5, device=dev)), dict(positions=torch.zeros(1, dtype=torch.long, device=dev)), dict(k=k.float()), dict(k=k[:1]),
+                dict(q=q[..., :32], k=k[..., :32]), dict(positions=torch.zeros(5, dtype=torch.bool, device=dev))):
+        with pytest.raises(ValueError):
+            ops.rope_qk(**{**dict(q=q, k=k, cos=cos, sin=sin), **bad})
+    ops.rope_qk(q, k, cos, sin)[0].float().sum().backward()
+    assert bool(torch.isfinite(cos.grad[:5]).all()) and not bool(cos.grad[5:].any())
+
+
 @pytest.mark.gpu
 def test_many_tokens():
     """More tokens than one pass of the grid has threads for: each CTA takes several turns."""
