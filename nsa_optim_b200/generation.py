@@ -108,6 +108,7 @@ class CacheStep:
         self.cache, self.plan, self.max_new = cache, plan, max_new
         self.limit = max(cache.held)                         # above all of the plan's positions, whatever leaves the cache later
         self._rotary: dict = {}
+        self._tables: dict = {}
 
     def __getitem__(self, layer: int):
         state = self.cache.layers[layer]
@@ -119,10 +120,21 @@ class CacheStep:
 
     def rotary(self, emb) -> Tuple[Tensor, Tensor]:
         """Cosines and sines of the step's positions, looked up once for all layers: for queries and keys that are turned outside of ``attend``."""
-        key = (emb.dim, emb.base, getattr(emb, "scaling", None))
+        key = self._angles(emb)
         if key not in self._rotary:
             self._rotary[key] = emb.rows(self.plan.positions, self.limit)
         return self._rotary[key]
+
+    def tables(self, emb) -> Tuple[Tensor, Tensor]:
+        """Tables that reach as far as the step, those of the first layer for all layers of the same angles: the others build none."""
+        key = self._angles(emb)
+        if key not in self._tables:
+            self._tables[key] = emb.tables(self.limit, self.plan.positions.device)
+        return self._tables[key]
+
+    @staticmethod
+    def _angles(emb):
+        return emb.dim, emb.base, getattr(emb, "scaling", None)
 
 
 class LayerStep:
@@ -138,7 +150,7 @@ class LayerStep:
         if rotary is None:
             ops.cache_append(self.pages, k, v, c.table, p.query_start, p.lengths)
         else:
-            cos, sin = rotary.tables(self.step.limit, q.device)
+            cos, sin = self.step.tables(rotary)
             q = ops.cache_append_rope(self.pages, q, k, v, cos, sin, c.table, p.query_start, p.lengths, rotary.interleaved)
         return ops.cache_attention(q, self.pages, c.table, p.query_start, p.lengths, max_new=self.step.max_new).unsqueeze(0)
 

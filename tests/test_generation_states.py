@@ -375,3 +375,16 @@ def test_layers_that_turn_by_themselves(dev, options):
     cache = PagedCache(model, requests=2, tokens=100, page_size=16)
     step = cache.step([2, 2])
     assert not torch.equal(step.rotary(RotaryEmbedding(64, 64, 1e4))[1], step.rotary(RotaryEmbedding(64, 64, 1e4, "linear:2"))[1])
+
+
+@pytest.mark.parametrize("hybrid", [False, True])
+def test_layers_share_the_rotary_tables(dev, hybrid):
+    """Generation builds the tables of one layer, not as many as there are layers."""
+    if hybrid:
+        model = small(dev, "AMA")
+    else:
+        model = placed(create_model(ModelConfig(name="small", hidden_size=128, intermediate_size=256, num_hidden_layers=3, num_attention_heads=4,
+                                                num_key_value_heads=2, head_dim=64, vocab_size=512, max_position_embeddings=32)), dev)
+    generate(model, texts([40, 3]), 30)
+    tables = [m for m in model.modules() if isinstance(m, RotaryEmbedding)]
+    assert len(tables) > 1 and [m.max_seq_len_cached >= 70 for m in tables] == [True] + [False] * (len(tables) - 1)
