@@ -103,7 +103,10 @@ __global__ void __launch_bounds__(kThreads) conv_cached_kernel(const bf16* __res
       const bf16* at = x + static_cast<long>(i) * ldx + c;
       if (t > 0) {
 #pragma unroll
-        for (int j = 0; j < K; ++j) h[j].load(at - (K - j) * ldx);
+        for (int j = 0; j < K; ++j) {
+          if (t >= K - j) h[j].load(at - (K - j) * ldx);
+          else h[j].zero();                                            // requests that overlap, which no step has: nothing in front of x is read
+        }
       } else {
         const bool fresh = r.length <= r.next - r.first;
         bf16* own = state + static_cast<long>(r.b) * K * C + c;
