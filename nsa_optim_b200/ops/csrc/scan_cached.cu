@@ -114,9 +114,10 @@ __device__ __forceinline__ void find_prompts(const Scan& a, int longest, const P
     const int b = base + t, n = b < a.B ? new_tokens(a, b) : 0;
     const int at = found + prefix256(n > longest, total, warps);
     found += total;
-    const int chunk = chunks + prefix256(n > longest ? (n + kChunk - 1) / kChunk : 0, total, warps);
+    const bool ours = n > longest && at < plan.room;                   // all of them, where requests do not overlap
+    const int chunk = chunks + prefix256(ours ? (n + kChunk - 1) / kChunk : 0, total, warps);
     chunks += total;
-    if (n > longest && at < plan.room) {
+    if (ours) {
       const int2 r = make_int2(b, min(chunk, plan.chunks));
       if (at < kRanked) requests[at] = r, sizes[at] = n;
       plan.requests()[at] = r;
