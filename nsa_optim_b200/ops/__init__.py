@@ -363,7 +363,7 @@ def conv1d_cached(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: Tens
                   activation: bool = True) -> Tensor:
     """:func:`causal_conv1d` of packed tokens (N, C) that continue their requests: the last ``query_start[b + 1] - query_start[b]`` of each request's
     ``lengths[b]`` tokens, after the inputs that its row of ``state`` (B, W - 1, C) holds (zeros where all of its tokens are new), which is brought up to date in
-    place.  Rows of no request give zeros.  Inference only.  bf16 with 2 to 4 taps on a GPU is a kernel; the rest runs in PyTorch, request by
+    place.  Rows of no request give zeros.  Inference only: results have no gradient.  bf16 with 2 to 4 taps on a GPU is a kernel; the rest runs in PyTorch, request by
     request, and waits for the device."""
     if _use_native(x, "causal_conv1d"):
         return native_module().conv1d_cached(x, weight, bias, state, query_start, lengths, activation)
@@ -375,9 +375,11 @@ def ssd_scan_cached(x: Tensor, dt: Tensor, A_log: Tensor, Bm: Tensor, Cm: Tensor
     """:func:`ssd_scan` of packed tokens that continue their requests, with the step sizes formed on the way: x (N, H, P), dt (N, H) as the projection gives
     it, B and C (N, G, S) for G groups of heads, A_log, dt_bias and D (H; D may be None).  The state of each head (B, H, P, S), fp32, is brought up to date in
     place; requests all of whose tokens are new begin from zeros.  Rows of no request give zeros.  ``max_new``, the most new tokens of a request, is a hint for the
-    choice of kernels (None: the number of tokens): any value gives the same sums up to their rounding.  What is not finite
-    stays in its request, whose rows it may reach up to 127 tokens back.  Inference only.  bf16 with 16, 32, 64, 128 or 256 states
-    on a GPU are kernels; the rest runs in PyTorch, request by request, and waits for the device."""
+    choice of kernels (None: the number of tokens): any value gives the same sums up to their rounding.  Up to 16 all of it is fp32; above, requests of more new
+    tokens than that (heads of 64 columns, 128 states) are products of bf16 operands: the state stays fp32, each term of a row is rounded once to 2^-8 of it, and
+    19.3 KB of scratch are taken for 128 tokens and head.  What is not finite stays in its request, whose rows it may reach up to 127 tokens back.  Inference only:
+    results have no gradient.  bf16 with 16, 32, 64, 128 or 256 states on a GPU are kernels; the rest runs in PyTorch, request by request, and waits for the
+    device."""
     if _use_native(x, "ssd_scan"):
         return native_module().ssd_scan_cached(x, dt, A_log, Bm, Cm, D, dt_bias, state, query_start, lengths, max_new)
     return states.scan(x, dt, A_log, Bm, Cm, D, dt_bias, state, query_start, lengths)

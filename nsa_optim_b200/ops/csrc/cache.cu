@@ -300,7 +300,7 @@ __device__ __forceinline__ void turn_block(Block<C>& x, const Turning& z, long b
     if (t0 + t >= from && t0 + t < to) turn_columns<C, MODE>(x.w[t], z, base + t0 + t, d);
 }
 // Queries of a window of tokens, heads h0 .. h1.  The tokens' positions are looked up first; then a thread has 2 V columns of a head at a time, two pieces of
-// V (their halves, or neighbours), and four heads or tokens in flight.
+// V (their halves, or neighbours), and two heads or tokens in flight.
 constexpr int kMostWindow = 256;
 template <int MODE, int V>
 __device__ __forceinline__ void turn_queries(const bf16* __restrict__ q, long ldq, bf16* __restrict__ y, const Turning& z, const CacheStep& s, int Hq, int h0,
@@ -456,7 +456,8 @@ __device__ __forceinline__ void store_values(uint8_t* codes, const Block<C>& x, 
 }
 
 // MODE other than kAsIs: keys are turned on the way, and the CTAs behind those of a window's keys and values turn its queries, kQueryHeads heads each: the
-// ones wait for their groups, the others for memory.  31.7 K tokens of 32 query and 8 cache heads of 128 (714 MB) 155 us, 4.6 TB/s; with all windows of keys
+// ones wait for their groups, the others for memory.  (A block's 16 tokens are turned in a loop that indexes them, so that blocks lie in local memory, the values' too:
+// 64 bytes of C = 2 and 128 of C = 4 beside spills.)  31.7 K tokens of 32 query and 8 cache heads of 128 (714 MB) 155 us, 4.6 TB/s; with all windows of keys
 // and values first 167; with 2 / 8 / 16 heads of queries 163 / 160 / 182, with one or three of them in flight 155 and 157 and four 165, in 56 or 80 registers 165 and
 // 182.
 constexpr int kQueryHeads = 4;

@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(256, S == 256 ? 2 : 4) scan_tokens_kernel(cons
 //     y_i = sum_{j <= i} (C_i . B_j) exp(c_i - c_j) d_j x_j + exp(c_i) C_i H + D x_i                            (scan_rows_kernel)
 // The first kernel walks the chunks of a request's head with the state in registers, from the request's own state and back to it, and leaves the state in
 // front of each chunk in bf16; the second has all chunks at once.  Operands of the rows' products are bf16 (scores and states are rounded to it), as where
-// the scan trains.  The state itself is fp32 and is handed on, so nothing is lost there: scaled x goes into its product as three bf16 numbers that add up
+// the scan trains: a rounding of 2^-8 in each term of a row, as in the row itself, that a hint of 16 new tokens at most avoids.  The state itself is fp32 and is handed on, so nothing is lost there: scaled x goes into its product as three bf16 numbers that add up
 // to it exactly.  Its weights come from sums that run back from the chunk's end: differences c_last - c_j would lose the last tokens' bits where c is large.
 
 // `bytes` consecutive bytes to shared memory; addresses and size are multiples of 16
@@ -655,8 +655,8 @@ struct Items {
 // columns each in front of the block, two those of the block itself, of even and odd items (their exponentials take twice as long), and two finish the
 // block's rows.  Two of the warps that are left issue products, and load and store.  C B^T stays in registers for all heads of a segment, the weights go to
 // tensor memory as the A operand, y leaves from the place of x.  Bound by memory and the handoffs of an item: one request of 16 K tokens and 64 heads
-// (402 MB) 71 us, 5.7 TB/s, 13.0 K in 8 (324 MB) 61; with warps that weigh an item and then finish the one before 88 and 76, with three stages of x and H
-// together 80, with a last chunk's rows stored one by one 75 for the eight.
+// (411 MB) 73 us, 5.6 TB/s, 13.0 K in 8 (331 MB) 62; before the sums had two numbers each 71 and 61, then with warps that weigh an item and then finish the one before 88 and 76, with three
+// stages of x and H together 80, with a last chunk's rows stored one by one 75 for the eight.
 constexpr int kRowsWarps = 28, kWeigh = 14, kFinish = 8, kIssue = 16, kCopy = 20;
 constexpr int kStages = 4, kStagesH = 3;               // of x and the sums, which stay until an item's rows are finished; of H, which its first product reads
 struct RowsSmem {
@@ -958,8 +958,9 @@ int tokens(const Scan& a, int longest, const Plan& plan, cudaStream_t st) {
 }
 
 // Requests of more new tokens than this go through the products, which read and write the states in front of chunks too but take 128 tokens about as fast as
-// one.  64 heads, requests of 8 / 16 / 24 / 32 / 64 tokens, token by token: one request 7.6 / 11.7 / 15.8 / 20.0 / 36.4 us, 8 requests 14.8 / 24.9 / 34.9 /
-// 44.9 / 86.7, 64 requests 98 / 161 / 226 / 290 / 547; by the products 19 / 19 / 18 / 18 / 17, 41 / 38 / 35 / 34 / 32 and 161 / 156 / 155 / 152 / 144.
+// one.  It is where both are alike for many requests, whose steps take longest; one request of 17 to 28 tokens loses up to 7 us by it, 8 of 17 to 23 up to 15.
+// 64 heads, requests of 8 / 16 / 24 / 32 / 64 tokens, token by token: one request 7.6 / 11.7 / 15.8 / 20.0 / 36.4 us, 8 requests 14.8 / 24.9 / 34.9 / 44.9 /
+// 86.7, 64 requests 98 / 161 / 226 / 290 / 547; by the products 19 / 19 / 18 / 18 / 17, 41 / 38 / 35 / 34 / 32 and 161 / 156 / 155 / 152 / 144.
 constexpr int kLongest = 16;
 
 Plan plan_of(int B, int N, int P, int S, int max_new) {
